@@ -285,6 +285,128 @@ int ifr_quant_gemm_ga(ifr_ctx* ctx, const ifr_dlinear* w, const int8_t* a_d, con
                       int32_t M, int32_t ga, float alpha, uint16_t* out_d);
 
 /* ------------------------------------------------------------------------
+ * A paged KV cache that the caller owns (no reference counterpart: its cache
+ * is a host array per layer, main.cpp:4286, with the narrower host codecs of
+ * :4406-4590).  For a program that keeps its own forward and pools: one pool
+ * of pages in device memory per layer, a plan per batch that all layers
+ * share, and three operators on them:
+ *   ifr_paged_append     new rows into the pages, K and Q rotated on the way
+ *   ifr_paged_attention  the new rows' attention over their sequences
+ *   ifr_paged_read       the new rows back as fp16 (cache export, tests)
+ * They run on the context's stream in call order and allocate nothing, so
+ * they can be captured into a graph; ifr_paged_set cannot (IFR_ESTATE), and
+ * a plan whose calls were captured refuses another ifr_paged_set, because
+ * the graph keeps that batch's launches.  Replays of graphs captured from
+ * one plan share its workspace: keep them on one stream.  The context's
+ * device is made current for the call and the caller's restored.
+ * ---------------------------------------------------------------------- */
+enum {
+  IFR_KV_FP16 = 0, /* fp16 */
+  IFR_KV_INT8 = 1, /* s = fp16(max|x| / 127) per (token, kv head), codes half
+                    * away from zero; a code stands for fp16(c s) */
+  IFR_KV_INT4 = 2  /* z = fp16(min), s = fp16((max - min) / 15) per (token, kv
+                    * head, 64 dims), codes rint((x - z) (1 / s)) in 0 .. 15;
+                    * a code stands for fp16(c s + z), rounded once */
+};
+/* A group of an 8- or 4-bit row that holds a NaN or an infinity reads back
+ * as NaN.  A page holds 32 tokens: per kv head one block
+ *   [K codes][K scales][V codes][V scales],
+ * heads in order, pages back to back, ifr_paged_bytes in all.  The element
+ * order inside a block is the order of the matrix instructions that read it,
+ * with hd = head_dim, token t and dim d:
+ *   K  fp16        element ((d / 8) * 32 + t) * 8 + d % 8
+ *      int8, int4  element ((t * 4 + d / 8 % 4) * (hd / 32) + d / 32) * 8 + d % 8
+ *   V  g = t % 16 / 4, j = 4 (t / 16) + t % 4
+ *      fp16        element (g * hd + d) * 8 + j
+ *      int8, int4  element ((g * 16 + d % 16) * (hd / 16) + d / 16) * 8 + j
+ *   int4: element e sits in nibble 4 (e % 2) + e % 8 / 2 of dword e / 8
+ *   fp16 scales, by index, u = d / 64:
+ *      int8  K (t % 16) * 2 + t / 16               V g * 8 + j
+ *      int4  K (((t % 16) * (hd / 64) + u) * 2 + t / 16) * 2, minimum + 1
+ *            V (g * (hd / 64) + u) * 16 + j,        minimum + 8
+ * Slots past a sequence's length are never looked at. */
+typedef struct ifr_paged_cfg {
+  int32_t format;   /* IFR_KV_* */
+  int32_t n_heads;  /* query heads, a multiple of n_kv */
+  int32_t n_kv;
+  int32_t head_dim; /* 64, 128 or 256 (else IFR_EDECLINE) */
+  int32_t n_pages;  /* pages of a pool */
+} ifr_paged_cfg;
+/* Bytes of one layer's pool (0 for a configuration that is refused).  A pool
+ * needs 16-byte alignment and no initialisation. */
+size_t ifr_paged_bytes(const ifr_paged_cfg* cfg);
+
+typedef struct ifr_paged ifr_paged;
+/* A plan belongs to its context and is destroyed before it. */
+int ifr_paged_create(ifr_ctx* ctx, const ifr_paged_cfg* cfg, ifr_paged** out);
+int ifr_paged_destroy(ifr_paged* p);
+
+/* One batch, in host memory (read during the call only).  Sequence s brings
+ * rows[s] new rows (0: it takes no part), which are its last positions, len[s]
+ * - rows[s] .. len[s] - 1; the batch's rows are those of sequence 0, then of
+ * sequence 1, and so on.  Entry i of a sequence's table row is the page of
+ * positions 32 i .. 32 i + 31; pages may be shared for reading, but a page
+ * that two sequences of the batch (or two entries of one) would write makes
+ * ifr_paged_append return IFR_EINVAL.
+ * A row at position pos sees the positions t with
+ *   first <= t < max(pos + 1, prefix),  t < len
+ * first: per row, the start of its document or window (NULL: 0); prefix: per
+ * sequence, a prefix that all of its rows see (NULL: 0).  A row that sees
+ * nothing gets zeros.  A batch that is refused with IFR_EINVAL leaves the
+ * plan as it was. */
+typedef struct ifr_paged_batch {
+  int32_t n_seqs;
+  const int32_t* rows;   /* [n_seqs] */
+  const int32_t* len;    /* [n_seqs] cached tokens, the new rows among them */
+  const int32_t* table;  /* [n_seqs][table_stride] */
+  int32_t table_stride;
+  const int32_t* first;  /* [rows of the batch] or NULL */
+  const int32_t* prefix; /* [n_seqs] or NULL */
+} ifr_paged_batch;
+int ifr_paged_set(ifr_paged* p, const ifr_paged_batch* b);
+
+/* Rows of a batch of M: fp16, row m at x_d + m * x_stride (in elements), heads
+ * back to back inside a row; 16-byte aligned, strides a multiple of 8 (slices
+ * of a fused QKV output qualify).  The rotation is rotate-half (rope,
+ * main.cpp:365-373) over the first `rotary` dims with the fp32 tables
+ * cos_d, sin_d [max_pos][rotary / 2], in fp32; K is stored from the fp32
+ * result.  Q is rotated into q_out_d, which is q_d itself (same stride) or
+ * overlaps nothing; both NULL: no Q. */
+typedef struct ifr_paged_rows {
+  const uint16_t* k_d; /* [M][n_kv][head_dim] */
+  const uint16_t* v_d;
+  int64_t k_stride, v_stride;
+  const uint16_t* q_d; /* [M][n_heads][head_dim] */
+  uint16_t* q_out_d;
+  int64_t q_stride, q_out_stride;
+  const float* cos_d;
+  const float* sin_d;
+  int32_t rotary;  /* a multiple of 16 up to head_dim; 0: no rotation */
+  int32_t max_pos; /* positions of the tables; more than the batch reaches */
+} ifr_paged_rows;
+int ifr_paged_append(ifr_paged* p, void* pool_d, const ifr_paged_rows* r);
+
+/* Attention of the batch's rows, whose K and V are in the pages already.  The
+ * score of position t is a = scale q.k, then cap tanh(a / cap) where softcap
+ * is set, then minus slopes[head] * |pos - t| where slopes are; softmax over
+ * the positions that the row sees. */
+typedef struct ifr_paged_query {
+  const uint16_t* q_d;  /* fp16 [M][n_heads][head_dim] */
+  int64_t q_stride;     /* elements, a multiple of 8 */
+  void* out_d;          /* fp16, or fp32 for ifr_act_quant; not q_d */
+  int64_t out_stride;   /* elements, a multiple of 16 bytes */
+  int32_t out_f32;      /* 0: fp16, 1: fp32 */
+  float scale;          /* 0: 1 / sqrt(head_dim) */
+  float softcap;        /* 0: none */
+  const float* slopes_d; /* fp32 [n_heads] or NULL */
+} ifr_paged_query;
+int ifr_paged_attention(ifr_paged* p, const void* pool_d, const ifr_paged_query* q);
+
+/* The batch's rows as the fp16 values that the cache holds for them:
+ * k_d, v_d [M][n_kv][head_dim], contiguous. */
+int ifr_paged_read(ifr_paged* p, const void* pool_d, uint16_t* k_d, uint16_t* v_d);
+
+/* ------------------------------------------------------------------------
  * Engine: model load, paged KV, one mixed iteration.
  * ---------------------------------------------------------------------- */
 typedef struct ifr_kv_cfg {

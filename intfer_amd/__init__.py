@@ -15,10 +15,10 @@ import numpy as np
 
 from . import _abi
 from ._abi import (KVCfg, Linear, ModelCfg, Row, SchedBackend, SchedCfg, ROW_DECODE, ROW_PREFILL,
-                   ROW_VERIFY, LIN_Q, LIN_K, LIN_V, LIN_O, LIN_GATE, LIN_UP, LIN_DOWN, IFR_OK, IFR_EDECLINE, IFR_EINVAL, IFR_ENOMEM, IFR_EDEVICE, IFR_ESTATE,
+                   ROW_VERIFY, KV_FP16, KV_INT8, KV_INT4, LIN_Q, LIN_K, LIN_V, LIN_O, LIN_GATE, LIN_UP, LIN_DOWN, IFR_OK, IFR_EDECLINE, IFR_EINVAL, IFR_ENOMEM, IFR_EDEVICE, IFR_ESTATE,
                    IfrError, check, lib)
 
-__all__ = ["Device", "Engine", "Scheduler", "Rng", "sample", "SynthModel", "HostModelHandle", "IntferFile", "default_cfg", "make_linear", "rows_array",
+__all__ = ["Device", "Engine", "Paged", "Scheduler", "KV_FP16", "KV_INT8", "KV_INT4", "Rng", "sample", "SynthModel", "HostModelHandle", "IntferFile", "default_cfg", "make_linear", "rows_array",
            "atile", "untile",
            "ROW_DECODE", "ROW_PREFILL", "ROW_VERIFY", "IfrError", "ModelCfg", "KVCfg", "SchedCfg",
            "Row", "Linear", "lib"]
@@ -437,6 +437,65 @@ class Engine:
         check(lib().ifr_get_timing(self.dev.ctx, kernel.encode(), C.byref(ms), C.byref(n),
                                    C.byref(b), C.byref(f)), "ifr_get_timing")
         return ms.value, n.value, b.value, f.value
+
+
+class Paged:
+    """The plan of a paged KV cache that the caller owns (ifr_paged_*): device
+    pointers are integers or c_void_p, strides count elements."""
+
+    def __init__(self, dev: Device, format: int, n_heads: int, n_kv: int, head_dim: int, n_pages: int):
+        self.dev, self.cfg, self.h = dev, _abi.PagedCfg(format, n_heads, n_kv, head_dim, n_pages), C.c_void_p()
+        check(lib().ifr_paged_create(dev.ctx, C.byref(self.cfg), C.byref(self.h)), "ifr_paged_create")
+
+    def pool_bytes(self) -> int:
+        """Bytes of one layer's pool."""
+        return lib().ifr_paged_bytes(C.byref(self.cfg))
+
+    def set(self, rows, lens, table, first=None, prefix=None):
+        """Per sequence: new rows, cached tokens (the new ones among them) and the
+        pages; optionally the first visible position of each row and a prefix of
+        each sequence."""
+        a = [None if x is None else np.ascontiguousarray(x, dtype=np.int32) for x in (rows, lens, table, first, prefix)]
+        S = len(a[0])
+        if len(a[1]) != S or a[2].ndim != 2 or a[2].shape[0] != S or (a[4] is not None and len(a[4]) != S):
+            raise ValueError("rows, lens, table and prefix name different numbers of sequences")
+        if a[3] is not None and len(a[3]) != int(a[0].sum()):
+            raise ValueError("first needs an entry for each row of the batch")
+        p = [None if x is None else x.ctypes.data_as(_abi.pi32) for x in a]
+        b = _abi.PagedBatch(S, p[0], p[1], p[2], a[2].shape[1], p[3], p[4])
+        check(lib().ifr_paged_set(self.h, C.byref(b)), "ifr_paged_set")
+
+    def append(self, pool, k, v, q=None, q_out=None, cos=None, sin=None, rotary=0, max_pos=0, k_stride=None,
+               v_stride=None, q_stride=None, q_out_stride=None):
+        """New rows into the pages; k and q rotated to their positions."""
+        c = self.cfg
+        kw, qw = c.n_kv * c.head_dim, c.n_heads * c.head_dim
+        r = _abi.PagedRows(k, v, k_stride or kw, v_stride or kw, q, q_out, q_stride or qw, q_out_stride or qw, cos, sin,
+                           rotary, max_pos)
+        check(lib().ifr_paged_append(self.h, pool, C.byref(r)), "ifr_paged_append")
+
+    def attention(self, pool, q, out, out_f32=False, scale=0.0, softcap=0.0, slopes=None, q_stride=None,
+                  out_stride=None):
+        """The new rows' attention over their sequences."""
+        qw = self.cfg.n_heads * self.cfg.head_dim
+        a = _abi.PagedQuery(q, q_stride or qw, out, out_stride or qw, int(out_f32), scale, softcap, slopes)
+        check(lib().ifr_paged_attention(self.h, pool, C.byref(a)), "ifr_paged_attention")
+
+    def read(self, pool, k, v):
+        """The new rows as the fp16 values that the cache holds."""
+        check(lib().ifr_paged_read(self.h, pool, k, v), "ifr_paged_read")
+
+    def close(self):
+        if self.h:
+            if self.dev.ctx:
+                lib().ifr_paged_destroy(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class Scheduler:

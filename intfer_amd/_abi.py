@@ -117,6 +117,29 @@ class SchedBackend(C.Structure):
                 ("seq_copy_prefix", SEQ_COPY), ("forward_logits", FORWARD_LOGITS), ("vocab", C.c_int32)]
 
 
+class PagedCfg(C.Structure):
+    _fields_ = [("format", C.c_int32), ("n_heads", C.c_int32), ("n_kv", C.c_int32), ("head_dim", C.c_int32),
+                ("n_pages", C.c_int32)]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [("n_seqs", C.c_int32), ("rows", C.POINTER(C.c_int32)), ("len", C.POINTER(C.c_int32)),
+                ("table", C.POINTER(C.c_int32)), ("table_stride", C.c_int32), ("first", C.POINTER(C.c_int32)),
+                ("prefix", C.POINTER(C.c_int32))]
+
+
+class PagedRows(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("q", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_int64), ("q_out_stride", C.c_int64),
+                ("cos", C.c_void_p), ("sin", C.c_void_p), ("rotary", C.c_int32), ("max_pos", C.c_int32)]
+
+
+class PagedQuery(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64),
+                ("out_f32", C.c_int32), ("scale", C.c_float), ("softcap", C.c_float), ("slopes", C.c_void_p)]
+
+
+KV_FP16, KV_INT8, KV_INT4 = 0, 1, 2
 P = C.c_void_p
 i32, i64, f32, sz = C.c_int32, C.c_int64, C.c_float, C.c_size_t
 pi32, pf32 = C.POINTER(C.c_int32), C.POINTER(C.c_float)
@@ -189,6 +212,13 @@ _PROTOS = {
     "ifr_linear_batch": (C.c_int, [P, i32, i32, pf32, pf32, i32]),
     "ifr_linear_wave_batch": (C.c_int, [P, C.POINTER(LinearItem), i32, i32]),
     "ifr_mlp_fused": (C.c_int, [P, i32, pf32, pf32, i32]),
+    "ifr_paged_bytes": (sz, [C.POINTER(PagedCfg)]),
+    "ifr_paged_create": (C.c_int, [P, C.POINTER(PagedCfg), C.POINTER(P)]),
+    "ifr_paged_destroy": (C.c_int, [P]),
+    "ifr_paged_set": (C.c_int, [P, C.POINTER(PagedBatch)]),
+    "ifr_paged_append": (C.c_int, [P, P, C.POINTER(PagedRows)]),
+    "ifr_paged_attention": (C.c_int, [P, P, C.POINTER(PagedQuery)]),
+    "ifr_paged_read": (C.c_int, [P, P, P, P]),
     "ifr_set_timing": (C.c_int, [P, i32]),
     "ifr_get_timing": (C.c_int, [P, C.c_char_p, C.POINTER(C.c_double), C.POINTER(i64),
                                  C.POINTER(C.c_double), C.POINTER(C.c_double)]),

@@ -30,7 +30,12 @@ SOURCES = [("qgemm.hip", [], "qgemm"),
            ("engine.cpp", [], "engine"), ("sched.cpp", [], "sched"), ("synth.cpp", [], "synth"),
            ("intfer_file.cpp", [], "intfer_file"), ("serve.cpp", [], "serve"),
            ("sample.cpp", [], "sample"), ("qgemm_f16.hip", [], "qgemm_f16"),
-           ("qgemm_ga.hip", [], "qgemm_ga"), ("peak.hip", [], "peak")]
+           ("qgemm_ga.hip", [], "qgemm_ga"), ("peak.hip", [], "peak"),
+           ("paged.cpp", [], "paged_plan"), ("paged.hip", [], "paged"), ("paged_attn.hip", [], "paged_attn"),
+           # the attention kernels of a caller's pages, once per cache format
+           ("paged_attn.hip", ["-DIFR_PAGED_FMT=0"], "paged_attn_f0"),
+           ("paged_attn.hip", ["-DIFR_PAGED_FMT=1"], "paged_attn_f1"),
+           ("paged_attn.hip", ["-DIFR_PAGED_FMT=2"], "paged_attn_f2")]
 SERVE_BIN = HERE / "intfer_serve"  # the --serve command line (serve_main.cpp)
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -48,7 +53,8 @@ COMMON = [
 # microbenchmark too (its accumulators otherwise shuffle between AGPRs and
 # VGPRs every round, which serializes the MFMA pipe).
 EXTRA = {"qgemm.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"], "attn.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
-         "peak.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"]}
+         "peak.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
+         "paged_attn.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"]}
 
 
 def _compile(item) -> Path:

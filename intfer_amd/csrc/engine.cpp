@@ -818,6 +818,10 @@ int ifr_ctx_destroy(ifr_ctx* c) {
   return IFR_OK;
 }
 
+}  // extern "C"
+int ifrh::ctx_device(const ifr_ctx* c) { return c->device; }
+extern "C" {
+
 void* ifr_ctx_stream(ifr_ctx* c) { return c ? (void*)c->st : nullptr; }
 
 int ifr_timer_begin(ifr_ctx* c) {

@@ -31,4 +31,7 @@ ifr_host_model* adopt(OwnedModel* m);
 // Record the message ifr_last_error() returns on this thread; returns code.
 int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 
+// The device that a context was made for.
+int ctx_device(const ifr_ctx* c);
+
 }  // namespace ifrh

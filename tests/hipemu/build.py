@@ -36,7 +36,11 @@ UNITS = [("qgemm.hip", [], "qgemm"),
          ("engine.cpp", [], "engine"), ("sched.cpp", [], "sched"), ("synth.cpp", [], "synth"),
          ("intfer_file.cpp", [], "intfer_file"), ("serve.cpp", [], "serve"),
          ("sample.cpp", [], "sample"), ("qgemm_f16.hip", [], "qgemm_f16"),
-           ("qgemm_ga.hip", [], "qgemm_ga"), ("peak.hip", [], "peak")]
+           ("qgemm_ga.hip", [], "qgemm_ga"), ("peak.hip", [], "peak"),
+         ("paged.cpp", [], "paged_plan"), ("paged.hip", [], "paged"), ("paged_attn.hip", [], "paged_attn"),
+         ("paged_attn.hip", ["-DIFR_PAGED_FMT=0"], "paged_attn_f0"),
+         ("paged_attn.hip", ["-DIFR_PAGED_FMT=1"], "paged_attn_f1"),
+         ("paged_attn.hip", ["-DIFR_PAGED_FMT=2"], "paged_attn_f2")]
 
 FLAGS = ["-O1", "-g", "-fPIC", "-std=c++17", "-fsanitize=address", "-fno-omit-frame-pointer",
          "-ffp-contract=off", "-Wno-unused-command-line-argument", "-w",

@@ -189,6 +189,8 @@ inline int __float_as_int(float f) { int x; std::memcpy(&x, &f, 4); return x; }
 inline unsigned __float_as_uint(float f) { unsigned x; std::memcpy(&x, &f, 4); return x; }
 // v_exp_f32 (2^x); the host's exp2f stands in for the hardware approximation
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
+// v_rcp_f32
+#define __builtin_amdgcn_rcpf(x) (1.0f / (x))
 
 inline int emu_readlane(int v, int l) {
   const unsigned char* s = emu::wave_exchange(&v, 4, emu::kOpReadlane);
@@ -281,6 +283,12 @@ hipError_t hipStreamCreate(hipStream_t* s);
 hipError_t hipStreamCreateWithFlags(hipStream_t* s, unsigned flags);
 hipError_t hipStreamDestroy(hipStream_t s);
 hipError_t hipStreamSynchronize(hipStream_t s);
+// (nothing is ever captured here)
+enum hipStreamCaptureStatus { hipStreamCaptureStatusNone = 0, hipStreamCaptureStatusActive = 1 };
+inline hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus* s) {
+  *s = hipStreamCaptureStatusNone;
+  return hipSuccess;
+}
 hipError_t hipDeviceSynchronize();
 hipError_t hipEventCreate(hipEvent_t* e);
 hipError_t hipEventCreateWithFlags(hipEvent_t* e, unsigned flags);

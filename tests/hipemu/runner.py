@@ -753,6 +753,30 @@ def act_quant():
 
 
 @scenario
+def paged_rows():
+    """A caller-owned paged cache with few rows: every format and head size, ragged lengths, odd groups."""
+    import intfer_amd as ia
+    from tests.paged_check import run_case
+    dev, rng = ia.Device(0), np.random.default_rng(3)
+    case = lambda *a, **k: run_case(ia, dev, rng, *a, **k, say=say)  # noqa: E731
+    for fmt in (0, 1, 2):
+        case(fmt, 4, 2, 128, [1, 2, 1, 5], [1, 33, 64, 170])
+        case(fmt, 2, 2, 64, [1, 3], [95, 40], out_f32=True, rotary=32)
+        case(fmt, 8, 2, 256, [1, 4], [31, 67], cap=5.0, rotary=64)
+    case(2, 5, 1, 128, [3, 0, 1], [300, 40, 700], bias=True, prefix=[290, 0, 5], out_f32=True)
+    case(0, 3, 1, 64, [7, 6], [7, 50], cap=30.0, rotary=0,
+         first=np.array([0, 0, 2, 2, 9, 5, 5, 44, 44, 47, 47, 49, 50]))
+
+
+@scenario
+def paged_refusals():
+    """The calls that the paged cache refuses."""
+    import intfer_amd as ia
+    from tests.paged_check import refusals
+    refusals(ia, ia.Device(0))
+
+
+@scenario
 def intfer_load():
     """An .intfer image (container-form model, post = 2/C, mixed widths)
     loaded through ifr_model_load_intfer runs one prefill chunk like the
