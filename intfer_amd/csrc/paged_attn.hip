@@ -14,7 +14,7 @@
 // Places that a row does not see: their scores are replaced, not added to, and
 // pages that some row sees only in part ("edge" pages) take V with every token
 // that no column sees cleared; if a non-finite V is left there, its products
-// are added only to the columns that see it (fix_nonfinite).
+// are added only to the columns that see it.
 #include "ifr_dev.h"
 #include "ifr_paged.h"
 
@@ -133,6 +133,23 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t x) {  // of two fp16
   return ((x & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
 }
 
+// One V element: token paged_vtok(g, j), dim d.
+template <int HD, int FMT>
+__device__ __forceinline__ float v_at(const uint8_t* p, int g, int j, int d) {
+  const int e = paged_vrun(FMT, HD, g, d) * 8 + j;
+  if constexpr (FMT == IFR_KV_FP16) {
+    return ifrd::h2f(reinterpret_cast<const uint16_t*>(p)[e]);
+  } else if constexpr (FMT == IFR_KV_INT8) {
+    const _Float16 s = __builtin_bit_cast(_Float16, reinterpret_cast<const uint16_t*>(p + 32 * HD)[g * 8 + j]);
+    return (float)((_Float16)(float)(int8_t)p[e] * s);
+  } else {
+    const uint16_t* sc = reinterpret_cast<const uint16_t*>(p + 16 * HD) + (g * (HD / kPgGroup) + d / kPgGroup) * 16 + j;
+    const int n = (e & ~7) + paged_nibble(e & 7);
+    return (float)__builtin_elementwise_fma((_Float16)(float)((p[n >> 1] >> (4 * (n & 1))) & 15),
+                                            __builtin_bit_cast(_Float16, sc[0]), __builtin_bit_cast(_Float16, sc[8]));
+  }
+}
+
 __device__ __forceinline__ int wave_max_i(int v) {
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) v = max(v, __shfl_xor(v, m, 64));
@@ -141,22 +158,29 @@ __device__ __forceinline__ int wave_max_i(int v) {
 
 // ---- few columns: the four waves of a workgroup take every fourth page ------------------------
 //
-// A wave holds NT tiles of 16 columns.  K is double-buffered, V single: page
-// i + 1's K is in flight while page i is computed, its V once page i's second
-// product has read V(i).  At the end the waves' (m, l, O) meet in LDS.
-template <int HD, int FMT, int NT>
+// A wave holds NT tiles of 16 columns.  The next page's K is loaded once the
+// first product has read this one's, its V once the second product has.  At
+// the end the waves' (m, l, O) meet in LDS.
+//
+// HL: P enters the second product as an fp16 high + low pair (22 bits), for
+// outputs in fp32.  An fp16 output takes P rounded to fp16, which is off like
+// the output's own rounding and saves 5 % (64 rows of 2048 int4 tokens 60.2 ->
+// 57.3 us, 16 of 32000 160.6 -> 152.3).  Bound by its VALU work at 4 bits:
+// 13 operations turn a dword of codes into 8 values.  (Two K buffers and both
+// steps unrolled spilled at 192 VGPRs: 142.8 and 467 us.)
+template <int HD, int FMT, int NT, bool HL>
 __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, PagedPool kv) {
   constexpr int I = HD / 32, N = HD / 16, U = HD / kPgGroup;
   constexpr int W = FMT == IFR_KV_FP16 ? 4 : FMT == IFR_KV_INT8 ? 2 : 1;  // dwords of 8 elements
-  constexpr size_t kPart = paged_part(FMT, HD), kPageB = 0;
+  constexpr size_t kPart = paged_part(FMT, HD);
   constexpr int kCodes = FMT == IFR_KV_INT8 ? 32 * HD : 16 * HD;
-  (void)kPageB;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const PagedUnit un = a.units[blockIdx.x];
   const int G = kv.nq / kv.nkv;
   const bool mod = a.cap != 0.0f || a.slopes != nullptr;
   const float inv_cap = a.cap != 0.0f ? 1.0f / a.cap : 0.0f;
+  const float sl = mod ? 1.0f : a.scale * kLog2e;  // what turns a score into powers of two
 
   v8h qf[NT][I];
   int lo[NT], hi[NT], pos[NT], lo_max = 0, hi_min = 0x7FFFFFFF, lo_min = 0x7FFFFFFF, hi_max = 0;
@@ -201,112 +225,126 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, Page
     for (int n = 0; n < N; ++n) o[t][n] = (v4f){0.f, 0.f, 0.f, 0.f};
   }
 
-  struct KBuf {
+  struct {
     uint32_t k[2][I * W];
     uint32_t sz[FMT == IFR_KV_INT4 ? 2 * U : 1];  // int4 [u][h]: scale | minimum; int8: both tiles' scales
-  };
-  struct VBuf {
+  } kb;
+  struct {
     uint32_t v[N * W];
     uint32_t s[FMT == IFR_KV_INT4 ? U * 8 : 4];   // int4 [u]: 8 scales, 8 minima; int8: 8 scales
-  };
+  } vb;
   const int32_t* tab = a.table + un.tab;
   const size_t page_bytes = paged_page(FMT, HD, kv.nkv), head = (size_t)un.kvh * 2 * kPart;
   // every load is unconditional (the page clamped to the unit's last one)
-  auto block_of = [&](int i) { return kv.pool + (size_t)tab[min(i, un.p1 - 1)] * page_bytes + head; };
-  auto load_k = [&](KBuf& b, int i) {
-    const uint8_t* p = block_of(i);
+  auto block_of = [&](int i) -> const uint8_t* { return kv.pool + (size_t)tab[min(i, un.p1 - 1)] * page_bytes + head; };
+  auto load_k = [&](const uint8_t* p) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if constexpr (FMT == IFR_KV_FP16) {
 #pragma unroll
-        for (int k = 0; k < I; ++k) load_dwords<4>(p + ((4 * k + g) * 32 + 16 * h + c) * 16, &b.k[h][4 * k]);
+        for (int k = 0; k < I; ++k) load_dwords<4>(p + ((4 * k + g) * 32 + 16 * h + c) * 16, &kb.k[h][4 * k]);
       } else {
-        load_dwords<I * W>(p + ((16 * h + c) * 4 + g) * (I * W * 4), b.k[h]);
+        load_dwords<I * W>(p + ((16 * h + c) * 4 + g) * (I * W * 4), kb.k[h]);
       }
     }
-    if constexpr (FMT == IFR_KV_INT8) load_dwords<1>(p + kCodes + c * 4, b.sz);
-    if constexpr (FMT == IFR_KV_INT4) load_dwords<2 * U>(p + kCodes + c * (8 * U), b.sz);
+    if constexpr (FMT == IFR_KV_INT8) load_dwords<1>(p + kCodes + c * 4, kb.sz);
+    if constexpr (FMT == IFR_KV_INT4) load_dwords<2 * U>(p + kCodes + c * (8 * U), kb.sz);
   };
-  auto load_v = [&](VBuf& b, int i) {
-    const uint8_t* p = block_of(i) + kPart;
+  auto load_v = [&](const uint8_t* p) {
+    p += kPart;
     if constexpr (FMT == IFR_KV_FP16) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) load_dwords<4>(p + (g * HD + 16 * n + c) * 16, &b.v[4 * n]);
+      for (int n = 0; n < N; ++n) load_dwords<4>(p + (g * HD + 16 * n + c) * 16, &vb.v[4 * n]);
     } else {
-      load_dwords<N * W>(p + (g * 16 + c) * (N * W * 4), b.v);
-      load_dwords<(FMT == IFR_KV_INT4 ? U * 8 : 4)>(p + kCodes + g * (FMT == IFR_KV_INT4 ? U * 32 : 16), b.s);
+      load_dwords<N * W>(p + (g * 16 + c) * (N * W * 4), vb.v);
+      load_dwords<(FMT == IFR_KV_INT4 ? U * 8 : 4)>(p + kCodes + g * (FMT == IFR_KV_INT4 ? U * 32 : 16), vb.s);
     }
   };
-  auto k_sz = [&](const KBuf& b, int h, int k) -> uint32_t {
-    if constexpr (FMT == IFR_KV_INT8) return h ? b.sz[0] >> 16 : b.sz[0];
-    else if constexpr (FMT == IFR_KV_INT4) return b.sz[(k / 2) * 2 + h];
-    else return 0;
-  };
 
-  auto step = [&](const KBuf& kb, const VBuf& vb, int i) {
+  const int i0 = un.p0 + w;
+  const uint8_t *cur = nullptr, *nxt = nullptr;
+  if (i0 < un.p1) {
+    cur = block_of(i0);
+    nxt = block_of(i0 + 4);
+    load_k(cur);
+    load_v(cur);
+  }
+#pragma unroll 1
+  for (int i = i0; i < un.p1; i += 4) {
+    const uint8_t* after = block_of(i + 8);  // its table entry is there when it is wanted
     const int t0 = i * kPgTok;
-    v8h kf[2][I];
+    v4f s[NT][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int k = 0; k < I; ++k) kf[h][k] = k_values<FMT>(&kb.k[h][k * W], k_sz(kb, h, k));
+      for (int k = 0; k < I; ++k) {
+        uint32_t sz = 0;
+        if constexpr (FMT == IFR_KV_INT8) sz = h ? kb.sz[0] >> 16 : kb.sz[0];
+        if constexpr (FMT == IFR_KV_INT4) sz = kb.sz[(k / 2) * 2 + h];
+        const v8h kf = k_values<FMT>(&kb.k[h][k * W], sz);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (k == 0) s[t][h] = (v4f){0.f, 0.f, 0.f, 0.f};
+          s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[t][k], s[t][h], 0, 0, 0);
+        }
+      }
+    load_k(nxt);
     const bool inner = t0 >= lo_max && t0 + kPgTok <= hi_min;  // every column sees the whole page
     v8h phi[NT], plo[NT];
-    float alpha[NT];
     uint32_t seen[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      v4f s[2];
+      float x[8], mt = -INFINITY;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s[h] = (v4f){0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < 8; ++j) x[j] = s[t][j >> 2][j & 3];
+      if (mod) {
 #pragma unroll
-        for (int k = 0; k < I; ++k) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][k], qf[t][k], s[h], 0, 0, 0);
+        for (int j = 0; j < 8; ++j) {
+          x[j] *= a.scale;
+          if (a.cap != 0.0f) x[j] = capped(x[j], a.cap, inv_cap);
+          x[j] -= slope[t] * (float)abs(pos[t] - (t0 + 16 * (j >> 2) + 4 * g + (j & 3)));
+          x[j] *= kLog2e;
+        }
       }
-      float sv[8], mt = -INFINITY;
       seen[t] = 0xFFu;
+      if (!inner) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float v = s[j >> 2][j & 3] * a.scale;
-        const int tk = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
-        if (mod) {
-          if (a.cap != 0.0f) v = capped(v, a.cap, inv_cap);
-          v -= slope[t] * (float)abs(pos[t] - tk);
+        for (int j = 0; j < 8; ++j) {
+          const int tk = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
+          if (tk < lo[t] || tk >= hi[t]) {
+            x[j] = -INFINITY;
+            seen[t] &= ~(1u << j);
+          }
         }
-        v *= kLog2e;
-        if (!inner && (tk < lo[t] || tk >= hi[t])) {
-          v = -INFINITY;
-          seen[t] &= ~(1u << j);
-        }
-        sv[j] = v;
-        mt = fmaxf(mt, v);
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mt = fmaxf(mt, x[j]);
       mt = fmaxf(mt, ifrd::lane_xor<16>(mt));
-      mt = fmaxf(mt, ifrd::lane_xor<32>(mt));
-      const float m_new = fmaxf(m_run[t], mt);
-      const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-      alpha[t] = __builtin_amdgcn_exp2f(m_run[t] - m_use);
-      // P as an fp16 high + low pair (22 bits): V is exact, so O keeps the
-      // accuracy of fp32
-      float rs = 0.0f;
+      mt = fmaxf(mt, ifrd::lane_xor<32>(mt)) * sl;
+      // The reference point of a column's powers moves only when some column's
+      // maximum has passed its own by 2^8: P stays below 2^8 and O is rescaled
+      // in few pages.
+      if (!__all(!(mt > m_run[t] + 8.0f))) {
+        const float m_new = fmaxf(m_run[t], mt);
+        const float al = m_run[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[t] - m_new);
+        m_run[t] = m_new;
+        l_run[t] *= al;
+#pragma unroll
+        for (int n = 0; n < N; ++n) o[t][n] *= al;
+      }
+      const float mu = m_run[t] == -INFINITY ? 0.0f : m_run[t];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float p = __builtin_amdgcn_exp2f(sv[j] - m_use);
-        rs += p;
+        const float p = __builtin_amdgcn_exp2f(fmaf(x[j], sl, -mu));
+        l_run[t] += p;  // this lane's tokens; the groups meet at the end
         const _Float16 hh = (_Float16)p;
         phi[t][j] = hh;
-        plo[t][j] = (_Float16)(p - (float)hh);
+        if constexpr (HL) plo[t][j] = (_Float16)(p - (float)hh);
       }
-      l_run[t] = l_run[t] * alpha[t] + rs;  // this lane's tokens; the groups meet at the end
-      m_run[t] = m_new;
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-      if (!__all(alpha[t] == 1.0f))
-#pragma unroll
-        for (int n = 0; n < N; ++n) o[t][n] *= alpha[t];
-    // tokens of this lane's V runs that some column of the unit sees
+    // an edge page: V of tokens that no column sees and non-finite V are cleared
     u4 keep = {~0u, ~0u, ~0u, ~0u};
+    uint32_t bad = 0;
     if (!inner) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -321,57 +359,48 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, Page
       v8h vf = v_values<FMT>(&vb.v[n * W], &vb.s[u * S], &vb.s[u * S + (FMT == IFR_KV_INT4 ? 4 : 0)]);
       if (!inner) {
         u4 x = __builtin_bit_cast(u4, vf) & keep;
-        uint32_t bad = nonfinite2(x[0]) | nonfinite2(x[1]) | nonfinite2(x[2]) | nonfinite2(x[3]);
-        if (!__all(bad == 0)) {
-          // a cached infinity or NaN in an edge page: out of the product, and
-          // added to the columns that see its token
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t e = (x[j >> 1] >> (16 * (j & 1))) & 0xFFFFu;
-            const bool nf = (e & 0x7C00u) == 0x7C00u;
-            const float mine = nf ? ifrd::h2f((uint16_t)e) : 0.0f;
-            if (nf) x[j >> 1] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-            for (int gt = 0; gt < 4; ++gt) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float vv = __shfl(mine, gt * 16 + 4 * g + r, 64);
-                const int bv = __shfl((int)nf, gt * 16 + 4 * g + r, 64);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                  const float p = __shfl((float)phi[t][j] + (float)plo[t][j], gt * 16 + c, 64);
-                  const int sb = __shfl((int)(seen[t] >> j) & 1, gt * 16 + c, 64);
-                  if (bv && sb) o[t][n][r] += p * vv;
-                }
-              }
-            }
-          }
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t nf = nonfinite2(x[q]);
+          bad |= nf;
+          x[q] &= ~((nf >> 15) * 0xFFFFu);
         }
         vf = __builtin_bit_cast(v8h, x);
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, phi[t], o[t][n], 0, 0, 0);
-        o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, plo[t], o[t][n], 0, 0, 0);
+        if constexpr (HL) o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, plo[t], o[t][n], 0, 0, 0);
       }
     }
-  };
-
-  const int i0 = un.p0 + w;
-  if (i0 < un.p1) {
-    KBuf ka, kb;
-    VBuf vb;
-    load_k(ka, i0);
-    load_v(vb, i0);
-    for (int i = i0;; i += 8) {
-      load_k(kb, i + 4);
-      step(ka, vb, i);
-      if (i + 4 >= un.p1) break;
-      load_v(vb, i + 4);
-      load_k(ka, i + 8);
-      step(kb, vb, i + 4);
-      if (i + 8 >= un.p1) break;
-      load_v(vb, i + 8);
+    load_v(nxt);
+    if (!__all(bad == 0)) {
+      // cached infinities or NaN where a column looks: their products, read
+      // again one by one, go to the columns that see them
+      const uint8_t* vp = cur + kPart;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll 1
+        for (int e = 0; e < 32; ++e) {
+          const int src = (e >> 3) * 16 + c, j = e & 7;
+          float pj = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (q == j) pj = (float)phi[t][q];
+          const float p = __shfl(pj, src, 64);
+          const int sb = __shfl((int)(seen[t] >> j) & 1, src, 64);
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float v = v_at<HD, FMT>(vp, e >> 3, j, 16 * n + 4 * g + r);
+              if (sb && (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) == 0x7F800000u) o[t][n][r] += p * v;
+            }
+        }
+      }
     }
+    cur = nxt;
+    nxt = after;
   }
 
   // ---- the four waves' parts: the columns' common maximum first, then O in
@@ -489,8 +518,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedJoin* joins,
 template <int HD, int FMT>
 hipError_t narrow_fmt(const PagedAttnArgs& a, const PagedPool& kv, int tiles, hipStream_t st) {
   const dim3 grid(a.n_units), block(256);
-  if (tiles == 1) hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, 1>), grid, block, 0, st, a, kv);
-  else if (tiles == 2) hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, 2>), grid, block, 0, st, a, kv);
+  if (tiles == 1 && a.out_f32) hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, 1, true>), grid, block, 0, st, a, kv);
+  else if (tiles == 1) hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, 1, false>), grid, block, 0, st, a, kv);
+  else if (tiles == 2 && a.out_f32) hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, 2, true>), grid, block, 0, st, a, kv);
+  else if (tiles == 2) hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, 2, false>), grid, block, 0, st, a, kv);
   else return hipErrorInvalidValue;
   return hipGetLastError();
 }

@@ -179,7 +179,9 @@ def attention(q, k, v, pos, lo, hi, scale, cap, slopes, out_f32):
     The bound: a score is a sum of hd products in fp32 and some 12 roundings after it (scale, cap, bias, the factor
     log2 e, the difference to the maximum), so it is off by (hd + 12) eps of the sum of its terms' magnitudes; exp2
     adds two steps and the fp16 pair of a weight 2^-22 of it or, below 2^-14 of the largest, 2^-25.  A weight that is
-    off by the factor 1 + e moves the output by at most 2 e sum p |v|.  Then the output's own rounding."""
+    off by the factor 1 + e moves the output by at most 2 e sum p |v|.  Then the output's own rounding.  For an fp16
+    output the weights of the numerator are rounded to fp16, each by at most 2^-11 of itself (the sum of the
+    denominator is not): at most 2^-11 sum p |v| more."""
     r, nq, hd = q.shape
     n, nkv = k.shape[:2]
     out, bound = np.zeros((r, nq, hd)), np.zeros((r, nq, hd))
@@ -206,6 +208,8 @@ def attention(q, k, v, pos, lo, hi, scale, cap, slopes, out_f32):
                 e = (hd + 12) * EPS32 * (size + np.abs(a) + np.abs(a.max())) + 2.0 ** -21
                 mean = (p * e).sum()
                 bound[i, h] = 2 * ((p * e) @ np.abs(vs) + mean * (p @ np.abs(vs))) + 2.0 ** -25 * np.abs(vs).sum(0) / w.sum()
+                if not out_f32:
+                    bound[i, h] += EPS16 * (p @ np.abs(vs))
     step = EPS32 if out_f32 else EPS16
     with np.errstate(all="ignore"):
         return out, bound + 2 * step * np.abs(out) + (0 if out_f32 else 2.0 ** -24)
