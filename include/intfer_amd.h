@@ -309,7 +309,8 @@ enum {
                     * a code stands for fp16(c s + z), rounded once */
 };
 /* A group of an 8- or 4-bit row that holds a NaN or an infinity reads back
- * as NaN.  A page holds 32 tokens: per kv head one block
+ * as NaN (its scale is NaN); of any other the scale is small enough for all
+ * codes to stand for finite values, which the attention relies on.  A page holds 32 tokens: per kv head one block
  *   [K codes][K scales][V codes][V scales],
  * heads in order, pages back to back, ifr_paged_bytes in all.  The element
  * order inside a block is the order of the matrix instructions that read it,

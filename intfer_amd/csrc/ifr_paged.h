@@ -108,6 +108,7 @@ struct PagedAttnArgs {
 // kPgWide columns.
 constexpr int kPgWide = 128;
 hipError_t launch_paged_narrow(const PagedAttnArgs& a, const PagedPool& kv, int tiles, hipStream_t st);
+hipError_t launch_paged_wide(const PagedAttnArgs& a, const PagedPool& kv, hipStream_t st);
 hipError_t launch_paged_join(const PagedJoin* joins, int n, const PagedAttnArgs& a, const PagedPool& kv,
                              hipStream_t st);
 

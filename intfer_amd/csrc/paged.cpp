@@ -30,10 +30,15 @@ namespace {
 constexpr int64_t kMaxRows = 1 << 24;      // rows of a batch
 constexpr int64_t kMaxTokens = 1 << 30;    // tokens of a sequence
 
+// Kinds of attention unit: narrow with one and two column tiles, wide.
+constexpr int kKinds = 3;
+constexpr int kWidth[kKinds] = {16, 32, ifrk::kPgWide};
+
 // Units that a batch is cut into at most when there is enough of it: four
-// workgroups for each of the 256 CUs.
-constexpr int64_t kUnits = 1024;
-constexpr int kMinPages = 4;  // a page for each wave of a narrow unit
+// narrow or two wide workgroups for each of the 256 CUs; and the fewest pages
+// of a split: a page for each wave of a narrow unit, 256 tokens of a wide one.
+constexpr int64_t kUnits[kKinds] = {1024, 1024, 512};
+constexpr int kMinPages[kKinds] = {4, 4, 8};
 
 // The context's device is current while a call runs, the caller's afterwards.
 struct OnDevice {
@@ -77,8 +82,8 @@ struct ifr_paged {
   size_t stage_cap = 0;
   hipEvent_t copied = nullptr;
   bool copying = false;
-  size_t o_rows = 0, o_runs = 0, o_units[2] = {0, 0}, o_joins = 0, o_table = 0;
-  int n_runs = 0, n_units[2] = {0, 0}, n_joins = 0;
+  size_t o_rows = 0, o_runs = 0, o_units[kKinds] = {}, o_joins = 0, o_table = 0;
+  int n_runs = 0, n_units[kKinds] = {}, n_joins = 0;
   float* part = nullptr;     // [columns][hd], then [columns][2]
   int64_t part_cap = 0, part_cols = 0;
 };
@@ -86,7 +91,7 @@ struct ifr_paged {
 namespace {
 
 struct Tile {
-  int seq, col0, ncol, p0, p1;
+  int kind, seq, col0, ncol, p0, p1;
 };
 
 int grow(ifr_paged* p, size_t meta, int64_t cols) {
@@ -150,7 +155,7 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
   std::vector<uint8_t> written((size_t)c.n_pages, 0);
   bool appendable = true;
   int max_pos = -1;
-  int64_t m = 0, pages = 0;
+  int64_t m = 0, pages[kKinds] = {};
   for (int s = 0; s < S; ++s) {
     const int n = b->len[s], r = b->rows[s];
     row0[s] = (int)m;
@@ -173,7 +178,7 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
       pos += k;
     }
     const int64_t ncols = (int64_t)r * G;
-    const int width = ncols <= 16 ? 16 : 32;
+    const int kind = ncols <= 16 ? 0 : ncols <= 32 ? 1 : 2, width = kWidth[kind];
     for (int64_t c0 = 0; c0 < ncols; c0 += width) {
       const int nc = (int)std::min<int64_t>(width, ncols - c0);
       int lo = 0x7FFFFFFF, hi = 0;
@@ -183,30 +188,33 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
         lo = std::min(lo, x.lo);
         hi = std::max(hi, x.hi);
       }
-      Tile tl{s, (int)c0, nc, 0, 0};
+      Tile tl{kind, s, (int)c0, nc, 0, 0};
       if (lo < hi) {
         tl.p0 = lo / kPgTok;
         tl.p1 = (hi + kPgTok - 1) / kPgTok;
       }
-      pages += tl.p1 - tl.p0;
+      pages[kind] += tl.p1 - tl.p0;
       tiles.push_back(tl);
     }
     m += r;
   }
-  const int64_t per = (pages * c.n_kv + kUnits - 1) / kUnits;
-  const int want = (int)std::max<int64_t>(kMinPages, (per + 3) / 4 * 4);
-  std::vector<ifrk::PagedUnit> units[2];
+  int wants[kKinds];
+  for (int k = 0; k < kKinds; ++k) {
+    const int64_t per = (pages[k] * c.n_kv + kUnits[k] - 1) / kUnits[k];
+    wants[k] = (int)std::max<int64_t>(kMinPages[k], (per + 3) / 4 * 4);
+  }
+  std::vector<ifrk::PagedUnit> units[kKinds];
   std::vector<ifrk::PagedJoin> joins;
   int64_t cols = 0;
   for (const Tile& t : tiles) {
-    const int np = t.p1 - t.p0, cuts = std::max(1, (np + want - 1) / want);
+    const int want = wants[t.kind], np = t.p1 - t.p0, cuts = std::max(1, (np + want - 1) / want);
     const int step = cuts == 1 ? std::max(np, 1) : ((np + cuts - 1) / cuts + 3) / 4 * 4;
     const int ns = std::max(1, (np + step - 1) / step);
     for (int h = 0; h < c.n_kv; ++h) {
       const int64_t base = cols;
       for (int s = 0; s < ns; ++s) {
         const int p0 = t.p0 + s * step, p1 = std::min(t.p1, p0 + step);
-        units[t.ncol > 16].push_back({row0[t.seq], h, t.col0, t.ncol, tab[t.seq], p0, p1, ns == 1 ? -1 : (int)cols});
+        units[t.kind].push_back({row0[t.seq], h, t.col0, t.ncol, tab[t.seq], p0, p1, ns == 1 ? -1 : (int)cols});
         if (ns > 1) cols += t.ncol;
       }
       if (cols > kMaxTokens) return fail(IFR_EINVAL, "too many partial columns");
@@ -222,8 +230,8 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
     return o;
   };
   const size_t o_rows = room(rows.size() * sizeof(rows[0])), o_runs = room(runs.size() * sizeof(runs[0]));
-  const size_t o_u0 = room(units[0].size() * sizeof(ifrk::PagedUnit));
-  const size_t o_u1 = room(units[1].size() * sizeof(ifrk::PagedUnit));
+  size_t o_units[kKinds];
+  for (int k = 0; k < kKinds; ++k) o_units[k] = room(units[k].size() * sizeof(ifrk::PagedUnit));
   const size_t o_joins = room(joins.size() * sizeof(ifrk::PagedJoin)), o_table = room(table.size() * 4);
   p->set = false;
   if (int r = grow(p, at, cols)) return r;
@@ -234,8 +242,7 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
   };
   put(o_rows, rows.data(), rows.size() * sizeof(rows[0]));
   put(o_runs, runs.data(), runs.size() * sizeof(runs[0]));
-  put(o_u0, units[0].data(), units[0].size() * sizeof(ifrk::PagedUnit));
-  put(o_u1, units[1].data(), units[1].size() * sizeof(ifrk::PagedUnit));
+  for (int k = 0; k < kKinds; ++k) put(o_units[k], units[k].data(), units[k].size() * sizeof(ifrk::PagedUnit));
   put(o_joins, joins.data(), joins.size() * sizeof(ifrk::PagedJoin));
   put(o_table, table.data(), table.size() * 4);
   if (at) {
@@ -245,13 +252,13 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
   }
   p->o_rows = o_rows;
   p->o_runs = o_runs;
-  p->o_units[0] = o_u0;
-  p->o_units[1] = o_u1;
   p->o_joins = o_joins;
   p->o_table = o_table;
   p->n_runs = (int)runs.size();
-  p->n_units[0] = (int)units[0].size();
-  p->n_units[1] = (int)units[1].size();
+  for (int k = 0; k < kKinds; ++k) {
+    p->o_units[k] = o_units[k];
+    p->n_units[k] = (int)units[k].size();
+  }
   p->n_joins = (int)joins.size();
   p->part_cols = cols;
   p->M = (int)M;
@@ -446,10 +453,10 @@ int ifr_paged_attention(ifr_paged* p, const void* pool_d, const ifr_paged_query*
   a.part_o = p->part;
   a.part_ml = p->part ? p->part + p->part_cols * c.head_dim : nullptr;
   const ifrk::PagedPool kv = pool_of(p, pool_d);
-  for (int i = 0; i < 2; ++i) {
-    a.units = reinterpret_cast<const ifrk::PagedUnit*>(p->meta + p->o_units[i]);
-    a.n_units = p->n_units[i];
-    PGCHK(ifrk::launch_paged_narrow(a, kv, i + 1, p->st));
+  for (int k = 0; k < kKinds; ++k) {
+    a.units = reinterpret_cast<const ifrk::PagedUnit*>(p->meta + p->o_units[k]);
+    a.n_units = p->n_units[k];
+    PGCHK(k < 2 ? ifrk::launch_paged_narrow(a, kv, k + 1, p->st) : ifrk::launch_paged_wide(a, kv, p->st));
   }
   PGCHK(ifrk::launch_paged_join(reinterpret_cast<const ifrk::PagedJoin*>(p->meta + p->o_joins), p->n_joins, a, kv,
                                 p->st));

@@ -10,14 +10,16 @@
 //   int4  z = fp16(min), s = fp16((max - min) / 15) per (token, head, 64 dims),
 //         c = rint((x - z) * (1 / s)) in 0 .. 15; it stands for fp16(c s + z)
 // A group that holds a NaN or an infinity gets a NaN scale and reads back as
-// NaN; the codes of a group whose scale rounds to zero are zero.
+// NaN; the codes of a group whose scale rounds to zero are zero.  A scale whose
+// largest code would round to infinity is the next smaller one (int8: 515.5 at
+// most), so that no finite row reads back as infinite.
 #include "ifr_dev.h"
 #include "ifr_paged.h"
 
 namespace ifrk {
 namespace {
 
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+constexpr float kMaxHalf = 65504.0f;
 
 __device__ __forceinline__ bool finite_f(float x) {
   return (__builtin_bit_cast(uint32_t, x) & 0x7F800000u) != 0x7F800000u;
@@ -50,7 +52,7 @@ __device__ __forceinline__ void quantize8(const float (&x)[8], uint32_t (&code)[
     for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(x[e]));
     a = group_max<LPT>(a);
     bad = group_max<LPT>(bad);
-    scale = bad != 0.0f ? (uint16_t)0x7E00u : ifrd::f2h(a / 127.0f);
+    scale = bad != 0.0f ? (uint16_t)0x7E00u : ifrd::f2h(fminf(a / 127.0f, 515.5f));
     const float s = ifrd::h2f(scale);
     const float inv = s > 0.0f && bad == 0.0f ? 1.0f / s : 0.0f;
 #pragma unroll
@@ -68,8 +70,15 @@ __device__ __forceinline__ void quantize8(const float (&x)[8], uint32_t (&code)[
     hi = group_max<8>(hi);
     lo = -group_max<8>(-lo);
     bad = group_max<8>(bad);
-    scale = bad != 0.0f ? (uint16_t)0x7E00u : ifrd::f2h((hi - lo) / 15.0f);
-    zero = bad != 0.0f ? (uint16_t)0 : ifrd::f2h(lo);
+    lo = fminf(fmaxf(lo, -kMaxHalf), kMaxHalf);  // (a rotated value can pass fp16's range)
+    hi = fminf(fmaxf(hi, -kMaxHalf), kMaxHalf);
+    scale = ifrd::f2h((hi - lo) / 15.0f);
+    zero = ifrd::f2h(lo);
+    if (15.0f * ifrd::h2f(scale) + ifrd::h2f(zero) >= 65520.0f) scale -= 1;  // code 15 would round to infinity
+    if (bad != 0.0f) {
+      scale = 0x7E00u;
+      zero = 0u;
+    }
     const float s = ifrd::h2f(scale), z = ifrd::h2f(zero);
     const float inv = s > 0.0f && bad == 0.0f ? 1.0f / s : 0.0f;
 #pragma unroll

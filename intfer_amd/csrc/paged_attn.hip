@@ -12,11 +12,13 @@
 // from there on all formats are the same kernel.
 //
 // Places that a row does not see: their scores are replaced, not added to, and
-// pages that some row sees only in part ("edge" pages) take V with every token
-// that no column sees cleared; if a non-finite V is left there, its products
-// are added only to the columns that see it.
+// in pages that some row sees only in part ("edge" pages) V is cleared where no
+// column looks and where it is not finite; what a column sees of the latter
+// goes into that column's result alone.
 #include "ifr_dev.h"
 #include "ifr_paged.h"
+
+#include <type_traits>
 
 namespace ifrk {
 namespace {
@@ -24,6 +26,7 @@ namespace {
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -111,51 +114,159 @@ __device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t* w) {
   }
 }
 
-// cap tanh(a / cap) with errors relative to the result, so that small scores
-// keep their bits: tanh x = x (135135 + 17325 y + 378 y^2 + y^3) /
-// (135135 + 62370 y + 3150 y^2 + 28 y^3), y = x^2, the seventh convergent of
-// Lambert's continued fraction (below 2e-8 off for |x| < 1), and
-// 1 - 2 / (e^2x + 1) from there on.
-__device__ __forceinline__ float capped(float a, float cap, float inv_cap) {
-  const float x = a * inv_cap, y = x * x;
-  const float n = fmaf(fmaf(fmaf(y, 1.0f, 378.0f), y, 17325.0f), y, 135135.0f);
-  const float d = fmaf(fmaf(fmaf(28.0f, y, 3150.0f), y, 62370.0f), y, 135135.0f);
-  float r = a * n * __builtin_amdgcn_rcpf(d);
-  if (!(y < 1.0f)) {
-    const float e = __builtin_amdgcn_exp2f(fabsf(x) * (2.0f * kLog2e));
-    r = __builtin_copysignf(cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f)), a);
-    if (a != a) r = a;
+// What a score becomes: in x[C] q.k, out the score times log2 e.
+//
+// cap tanh(a / cap) keeps errors relative to the result, so that small scores
+// keep their bits.  While every |a / cap| of the wave is at most 1/2 (scores
+// hardly ever come near their cap) it is x P(x^2), P the degree-4 Chebyshev
+// interpolation of tanh(x) / x in x^2 on [0, 1/4] (1.4e-8 off), 7 operations a
+// score; else 1 - 2 / (e^2x + 1) above 1/2.  The bias takes |pos - t| in fp32,
+// exact up to 2^24; far(j) is pos - t of score j.
+struct Scoring {
+  float scale2;           // scale log2 e
+  float inv, cap2;        // scale / cap, cap log2 e; inv 0: no cap
+  bool mod;               // cap or bias
+};
+__device__ __forceinline__ Scoring scoring(const PagedAttnArgs& a) {
+  Scoring s;
+  s.scale2 = a.scale * kLog2e;
+  s.inv = a.cap != 0.0f ? a.scale / a.cap : 0.0f;
+  s.cap2 = a.cap * kLog2e;
+  s.mod = a.cap != 0.0f || a.slopes != nullptr;
+  return s;
+}
+template <int C, typename Far>
+__device__ __forceinline__ void modify(float (&x)[C], const Scoring& s, bool biased, float slope2, Far far) {
+  if (s.inv != 0.0f) {
+    float big = 0.0f;
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      x[j] *= s.inv;
+      big = fmaxf(big, fabsf(x[j]));
+    }
+    auto poly = [](float v) {
+      const float y = v * v;
+      return v * fmaf(fmaf(fmaf(fmaf(0.0171313444f, y, -0.0529842388f), y, 0.133247505f), y, -0.333330679f), y, 0.99999999f);
+    };
+    if (__all(!(big > 0.5f))) {
+#pragma unroll
+      for (int j = 0; j < C; ++j) x[j] = poly(x[j]) * s.cap2;
+    } else {
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const float e = __builtin_amdgcn_exp2f(fabsf(x[j]) * (2.0f * kLog2e));
+        const float t = __builtin_copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f), x[j]);
+        x[j] = (fabsf(x[j]) > 0.5f ? t : poly(x[j])) * s.cap2;
+        __builtin_amdgcn_sched_barrier(0);  // (one at a time: the seldom case is to hold few registers)
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < C; ++j) x[j] *= s.scale2;
   }
-  return r;
+  if (biased) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) x[j] = fmaf(-slope2, fabsf(far(j)), x[j]);
+  }
 }
 
 __device__ __forceinline__ uint32_t nonfinite2(uint32_t x) {  // of two fp16
   return ((x & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
 }
 
-// One V element: token paged_vtok(g, j), dim d.
-template <int HD, int FMT>
-__device__ __forceinline__ float v_at(const uint8_t* p, int g, int j, int d) {
-  const int e = paged_vrun(FMT, HD, g, d) * 8 + j;
-  if constexpr (FMT == IFR_KV_FP16) {
-    return ifrd::h2f(reinterpret_cast<const uint16_t*>(p)[e]);
-  } else if constexpr (FMT == IFR_KV_INT8) {
-    const _Float16 s = __builtin_bit_cast(_Float16, reinterpret_cast<const uint16_t*>(p + 32 * HD)[g * 8 + j]);
-    return (float)((_Float16)(float)(int8_t)p[e] * s);
-  } else {
-    const uint16_t* sc = reinterpret_cast<const uint16_t*>(p + 16 * HD) + (g * (HD / kPgGroup) + d / kPgGroup) * 16 + j;
-    const int n = (e & ~7) + paged_nibble(e & 7);
-    return (float)__builtin_elementwise_fma((_Float16)(float)((p[n >> 1] >> (4 * (n & 1))) & 15),
-                                            __builtin_bit_cast(_Float16, sc[0]), __builtin_bit_cast(_Float16, sc[8]));
-  }
-}
-
-__device__ __forceinline__ int wave_max_i(int v) {
+__device__ __forceinline__ int wave_max_i(int v) {  // uniform, in a scalar register
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) v = max(v, __shfl_xor(v, m, 64));
-  return v;
+  return __builtin_amdgcn_readfirstlane(v);
 }
-
+// ---- V of edge pages ----
+// Tokens that no column sees are cleared, and so are values that are not
+// finite: a product with a weight of zero must stay zero.  What a column does
+// see of the latter is noted per element of O (Unbounded) and put into the
+// result.  fp16 is judged value by value, a quantized token by its scale.
+template <int FMT>
+__device__ __forceinline__ bool not_finite(uint32_t s, uint32_t z) {  // (low halves)
+  return (s & 0x7C00u) == 0x7C00u || (FMT == IFR_KV_INT4 && (z & 0x7C00u) == 0x7C00u);
+}
+// fp16: a run of 8 tokens
+__device__ __forceinline__ void edge_run(uint32_t* x, const u4& keep, uint32_t& bad) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    x[q] &= keep[q];
+    const uint32_t nf = nonfinite2(x[q]);
+    bad |= nf;
+    x[q] &= ~((nf >> 15) * 0xFFFFu);
+  }
+}
+// int8, int4: the scales (and minima) of 8 tokens
+template <int FMT>
+__device__ __forceinline__ void edge_scales(uint32_t* s, uint32_t* z, const u4& keep, uint32_t& bad) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    s[q] &= keep[q];
+    uint32_t nf = nonfinite2(s[q]);
+    if constexpr (FMT == IFR_KV_INT4) {
+      z[q] &= keep[q];
+      nf |= nonfinite2(z[q]);
+    }
+    bad |= nf;
+    const uint32_t in = ~((nf >> 15) * 0xFFFFu);
+    s[q] &= in;
+    if constexpr (FMT == IFR_KV_INT4) z[q] &= in;
+  }
+}
+// Elements of a lane's O that got +infinity, -infinity (both: NaN).
+template <int N>
+struct Unbounded {
+  uint64_t up[(N + 63) / 64], down[(N + 63) / 64];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < (N + 63) / 64; ++i) up[i] = down[i] = 0;
+  }
+  // V element (group g, element j, dim d) of the part p, seen by this lane's column, to element k
+  template <int HD, int FMT>
+  __device__ __forceinline__ void add(const uint8_t* p, int g, int j, int d, int k) {
+    bool hi, lo;
+    if constexpr (FMT == IFR_KV_FP16) {
+      const uint32_t x = reinterpret_cast<const uint16_t*>(p)[paged_vrun(FMT, HD, g, d) * 8 + j];
+      const bool nan = (x & 0x7FFFu) > 0x7C00u;
+      hi = x == 0x7C00u || nan;
+      lo = x == 0xFC00u || nan;
+    } else {
+      constexpr int kCodes = FMT == IFR_KV_INT8 ? 32 * HD : 16 * HD;
+      const uint16_t* sc = reinterpret_cast<const uint16_t*>(p + kCodes) +
+                           (FMT == IFR_KV_INT8 ? g * 8 + j : (g * (HD / kPgGroup) + d / kPgGroup) * 16 + j);
+      hi = lo = not_finite<FMT>(sc[0], FMT == IFR_KV_INT4 ? sc[8] : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < (N + 63) / 64; ++i) {
+      const uint64_t bit = k / 64 == i ? (uint64_t)1 << (k & 63) : 0;
+      if (hi) up[i] |= bit;
+      if (lo) down[i] |= bit;
+    }
+  }
+  __device__ __forceinline__ bool any() const {
+    uint64_t x = 0;
+#pragma unroll
+    for (int i = 0; i < (N + 63) / 64; ++i) x |= up[i] | down[i];
+    return x != 0;
+  }
+  __device__ __forceinline__ float value(int k, float x) const {
+    if ((up[k / 64] >> (k & 63)) & 1) x += INFINITY;
+    if ((down[k / 64] >> (k & 63)) & 1) x -= INFINITY;
+    return x;
+  }
+};
+// Tokens of lane group g's run (from position t0) that lie in [lo, hi)
+__device__ __forceinline__ u4 kept(int t0, int g, int lo, int hi) {
+  u4 keep = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int t = t0 + paged_vtok(g, j);
+    if (t >= lo && t < hi) keep[j >> 1] |= j & 1 ? 0xFFFF0000u : 0x0000FFFFu;
+  }
+  return keep;
+}
 // ---- few columns: the four waves of a workgroup take every fourth page ------------------------
 //
 // A wave holds NT tiles of 16 columns.  The next page's K is loaded once the
@@ -168,8 +279,14 @@ __device__ __forceinline__ int wave_max_i(int v) {
 // 57.3 us, 16 of 32000 160.6 -> 152.3).  Bound by its VALU work at 4 bits:
 // 13 operations turn a dword of codes into 8 values.  (Two K buffers and both
 // steps unrolled spilled at 192 VGPRs: 142.8 and 467 us.)
+// (waves a SIMD: what the registers of o, q and the raw page allow)
+constexpr int narrow_waves(int fmt, int hd, int nt) {
+  if (fmt == IFR_KV_FP16 && hd >= 128) return hd == 128 ? 2 : 1;
+  return hd * nt <= 64 ? 4 : hd * nt <= 128 ? 3 : hd * nt <= 256 ? 2 : 1;
+}
+
 template <int HD, int FMT, int NT, bool HL>
-__global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, PagedPool kv) {
+__global__ __launch_bounds__(256, narrow_waves(FMT, HD, NT)) void paged_narrow_kernel(PagedAttnArgs a, PagedPool kv) {
   constexpr int I = HD / 32, N = HD / 16, U = HD / kPgGroup;
   constexpr int W = FMT == IFR_KV_FP16 ? 4 : FMT == IFR_KV_INT8 ? 2 : 1;  // dwords of 8 elements
   constexpr size_t kPart = paged_part(FMT, HD);
@@ -178,9 +295,8 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, Page
   const int c = lane & 15, g = lane >> 4;
   const PagedUnit un = a.units[blockIdx.x];
   const int G = kv.nq / kv.nkv;
-  const bool mod = a.cap != 0.0f || a.slopes != nullptr;
-  const float inv_cap = a.cap != 0.0f ? 1.0f / a.cap : 0.0f;
-  const float sl = mod ? 1.0f : a.scale * kLog2e;  // what turns a score into powers of two
+  const Scoring sco = scoring(a);
+  const float sl = sco.mod ? 1.0f : sco.scale2;  // what turns a score into powers of two
 
   v8h qf[NT][I];
   int lo[NT], hi[NT], pos[NT], lo_max = 0, hi_min = 0x7FFFFFFF, lo_min = 0x7FFFFFFF, hi_max = 0;
@@ -196,7 +312,7 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, Page
     lo[t] = max(r.lo, un.p0 * kPgTok);
     hi[t] = on[t] ? min(r.hi, un.p1 * kPgTok) : 0;
     pos[t] = r.pos;
-    slope[t] = a.slopes ? a.slopes[h] : 0.0f;
+    slope[t] = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
     if (on[t]) {
       lo_max = max(lo_max, lo[t]);
       hi_min = min(hi_min, hi[t]);
@@ -224,6 +340,9 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, Page
 #pragma unroll
     for (int n = 0; n < N; ++n) o[t][n] = (v4f){0.f, 0.f, 0.f, 0.f};
   }
+  Unbounded<4 * N> ub[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) ub[t].clear();
 
   struct {
     uint32_t k[2][I * W];
@@ -275,7 +394,8 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, Page
     const int t0 = i * kPgTok;
     v4f s[NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
+      if (h) __builtin_amdgcn_sched_barrier(0);  // (the scheduler would keep every value of the page in registers)
 #pragma unroll
       for (int k = 0; k < I; ++k) {
         uint32_t sz = 0;
@@ -288,6 +408,7 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, Page
           s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[t][k], s[t][h], 0, 0, 0);
         }
       }
+    }
     load_k(nxt);
     const bool inner = t0 >= lo_max && t0 + kPgTok <= hi_min;  // every column sees the whole page
     v8h phi[NT], plo[NT];
@@ -297,14 +418,9 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, Page
       float x[8], mt = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = s[t][j >> 2][j & 3];
-      if (mod) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] *= a.scale;
-          if (a.cap != 0.0f) x[j] = capped(x[j], a.cap, inv_cap);
-          x[j] -= slope[t] * (float)abs(pos[t] - (t0 + 16 * (j >> 2) + 4 * g + (j & 3)));
-          x[j] *= kLog2e;
-        }
+      if (sco.mod) {
+        const float d = (float)(pos[t] - t0 - 4 * g);
+        modify(x, sco, a.slopes != nullptr, slope[t], [&](int j) { return d - (float)(16 * (j >> 2) + (j & 3)); });
       }
       seen[t] = 0xFFu;
       if (!inner) {
@@ -342,31 +458,22 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, Page
         if constexpr (HL) plo[t][j] = (_Float16)(p - (float)hh);
       }
     }
-    // an edge page: V of tokens that no column sees and non-finite V are cleared
-    u4 keep = {~0u, ~0u, ~0u, ~0u};
     uint32_t bad = 0;
+    constexpr int S = FMT == IFR_KV_INT4 ? 8 : 0;
     if (!inner) {
+      const u4 keep = kept(t0, g, lo_min, hi_max);
+      if constexpr (FMT == IFR_KV_FP16) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int tk = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
-        if (tk < lo_min || tk >= hi_max) keep[j >> 1] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+        for (int n = 0; n < N; ++n) edge_run(&vb.v[4 * n], keep, bad);
+      } else {
+#pragma unroll
+        for (int u = 0; u < (S ? U : 1); ++u) edge_scales<FMT>(&vb.s[u * S], &vb.s[u * S + S / 2], keep, bad);
       }
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      constexpr int S = FMT == IFR_KV_INT4 ? 8 : 0;
       const int u = n / 4;
-      v8h vf = v_values<FMT>(&vb.v[n * W], &vb.s[u * S], &vb.s[u * S + (FMT == IFR_KV_INT4 ? 4 : 0)]);
-      if (!inner) {
-        u4 x = __builtin_bit_cast(u4, vf) & keep;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t nf = nonfinite2(x[q]);
-          bad |= nf;
-          x[q] &= ~((nf >> 15) * 0xFFFFu);
-        }
-        vf = __builtin_bit_cast(v8h, x);
-      }
+      const v8h vf = v_values<FMT>(&vb.v[n * W], &vb.s[u * S], &vb.s[u * S + S / 2]);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, phi[t], o[t][n], 0, 0, 0);
@@ -374,34 +481,28 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, Page
       }
     }
     load_v(nxt);
-    if (!__all(bad == 0)) {
-      // cached infinities or NaN where a column looks: their products, read
-      // again one by one, go to the columns that see them
-      const uint8_t* vp = cur + kPart;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
+    if (!__all(bad == 0)) {  // rare: a cached infinity or NaN where some column looks
 #pragma unroll 1
-        for (int e = 0; e < 32; ++e) {
-          const int src = (e >> 3) * 16 + c, j = e & 7;
-          float pj = 0.0f;
+      for (int e = 0; e < 32; ++e) {  // group e / 8, element e % 8
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (q == j) pj = (float)phi[t][q];
-          const float p = __shfl(pj, src, 64);
-          const int sb = __shfl((int)(seen[t] >> j) & 1, src, 64);
-#pragma unroll
-          for (int n = 0; n < N; ++n)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float v = v_at<HD, FMT>(vp, e >> 3, j, 16 * n + 4 * g + r);
-              if (sb && (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) == 0x7F800000u) o[t][n][r] += p * v;
-            }
+        for (int t = 0; t < NT; ++t) {
+          const int sb = __shfl((int)(seen[t] >> (e & 7)) & 1, (e >> 3) * 16 + c, 64);
+          if (!sb) continue;
+#pragma unroll 1
+          for (int k = 0; k < 4 * N; ++k)
+            ub[t].template add<HD, FMT>(cur + kPart, e >> 3, e & 7, 16 * (k >> 2) + 4 * g + (k & 3), k);
         }
       }
     }
     cur = nxt;
     nxt = after;
   }
+
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    if (!__all(!ub[t].any()))
+#pragma unroll
+      for (int k = 0; k < 4 * N; ++k) o[t][k >> 2][k & 3] = ub[t].value(k, o[t][k >> 2][k & 3]);
 
   // ---- the four waves' parts: the columns' common maximum first, then O in
   // slices of 64 dims
@@ -470,6 +571,288 @@ __global__ __launch_bounds__(256) void paged_narrow_kernel(PagedAttnArgs a, Page
   }
 }
 
+// ---- many columns: the four waves of a workgroup take 32 columns each and share the pages ------
+//
+// The workgroup turns NP pages a step into fp16 in LDS, two buffers in turn:
+// the next step's codes are in flight while this one is computed, one barrier
+// a step.  32x32x16 MFMAs: K row rho of a page is token wide_tok(rho), so that
+// the scores a lane gets are the P elements that it holds of V's runs.  The
+// 16-byte runs of a dim block (K) or of 16 dims (V) are rotated against each
+// other by an exclusive or, which spreads both the quantized formats' stores
+// and the reads over the banks.
+__device__ __forceinline__ int wide_tok(int rho) {
+  return 8 * (rho >> 4) + 4 * ((rho >> 2) & 1) + 16 * ((rho >> 3) & 1) + (rho & 3);
+}
+__device__ __forceinline__ int wide_row(int t) {
+  return 16 * ((t >> 3) & 1) + 8 * (t >> 4) + 4 * ((t >> 2) & 1) + (t & 3);
+}
+__device__ __forceinline__ int k_run(int blk, int rho) { return blk * 32 + (rho ^ (blk & 15)); }
+template <int HD>
+__device__ __forceinline__ int v_run(int g, int d) { return g * HD + (d ^ ((d >> 4) & 15)); }
+
+template <int HD, int FMT, bool HL>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_wide_kernel(PagedAttnArgs a, PagedPool kv) {
+  constexpr int NP = HD == 256 ? 1 : 2;
+  constexpr int I = HD / 32, N = HD / 16, U = HD / kPgGroup, KS = HD / 16, D = HD / 32;
+  constexpr int RUNS = 4 * HD;  // 16-byte runs of a page's K (or V) in LDS
+  constexpr size_t kPart = paged_part(FMT, HD);
+  constexpr int kCodes = FMT == IFR_KV_INT8 ? 32 * HD : 16 * HD;
+  __shared__ __align__(16) u4 lds[2][2][NP * RUNS];  // [buffer][K, V]
+  __shared__ int aside[2];                           // step + 1 of the last one in this buffer that set V aside
+  __shared__ int range[4][4];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, hl = lane >> 5;
+  const PagedUnit un = a.units[blockIdx.x];
+  const int G = kv.nq / kv.nkv;
+  const Scoring sco = scoring(a);
+  const float sl = sco.mod ? 1.0f : sco.scale2;
+
+  // this lane's column
+  const int ci = 32 * w + c;
+  const bool on = ci < un.ncol;
+  const int col = un.col0 + (on ? ci : 0), row = un.row0 + col / G, h = un.kvh * G + col % G;
+  const PagedRow pr = a.rows[row];
+  const int lo = max(pr.lo, un.p0 * kPgTok), hi = on ? min(pr.hi, un.p1 * kPgTok) : 0, pos = pr.pos;
+  const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+  const int lo_max = wave_max_i(on ? lo : 0), hi_max = wave_max_i(on ? hi : 0);
+  const int hi_min = -wave_max_i(on ? -hi : -0x7FFFFFFF), lo_min = -wave_max_i(on ? -lo : -0x7FFFFFFF);
+  // ... and of the workgroup's columns
+  if (tid < 2) aside[tid] = 0;
+  if (lane == 0) {
+    range[w][0] = lo_min;
+    range[w][1] = -lo_max;
+    range[w][2] = -hi_max;
+    range[w][3] = hi_min;
+  }
+  __syncthreads();
+  auto least = [&](int i) {
+    return __builtin_amdgcn_readfirstlane(min(min(range[0][i], range[1][i]), min(range[2][i], range[3][i])));
+  };
+  const int wg_lo = least(0), wg_lo_max = -least(1), wg_hi = -least(2), wg_hi_min = least(3);
+  v8h qf[KS];
+  {
+    const uint16_t* qp = a.q + (int64_t)row * a.q_stride + (int64_t)h * HD + 8 * hl;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const v8h x = *reinterpret_cast<const v8h*>(qp + 16 * k);
+      qf[k] = on ? x : (v8h){0, 0, 0, 0, 0, 0, 0, 0};
+    }
+  }
+  float m_run = -INFINITY, l_run = 0.0f;
+  v16f o[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+  Unbounded<16 * D> ub;
+  ub.clear();
+
+  // ---- staging: what a thread holds of a step
+  constexpr int FR = FMT == IFR_KV_FP16 ? NP * RUNS / 256 : 1;
+  constexpr int KD = FMT == IFR_KV_INT8 ? 2 * I : I;              // dwords of a K item (token, group)
+  constexpr int VD = FMT == IFR_KV_INT8 ? 8 : 4;                  // dwords of a V item (group, c, 64 dims)
+  constexpr int K_ITEMS = NP * 128, V_ITEMS = NP * 64 * U;        // at most 256 each
+  struct {
+    u4 kf[FR], vf[FR];                                            // fp16
+    uint32_t k[KD], ks[FMT == IFR_KV_INT4 ? U : 1], v[VD], vs[8]; // int8, int4
+  } sg;
+  const int32_t* tab = a.table + un.tab;
+  const size_t page_bytes = paged_page(FMT, HD, kv.nkv), head = (size_t)un.kvh * 2 * kPart;
+  auto block_of = [&](int st, int ps) -> const uint8_t* {
+    return kv.pool + (size_t)tab[min(un.p0 + NP * st + ps, un.p1 - 1)] * page_bytes + head;
+  };
+  auto load_stage = [&](int st) {
+    if constexpr (FMT == IFR_KV_FP16) {
+#pragma unroll
+      for (int r = 0; r < FR; ++r) {
+        const int e = tid + 256 * r, ps = 256 * r / RUNS, i = e % RUNS;
+        const uint8_t* p = block_of(st, ps);
+        sg.kf[r] = reinterpret_cast<const u4*>(p)[(i & ~31) + wide_tok(i & 31)];
+        sg.vf[r] = reinterpret_cast<const u4*>(p + kPart)[i];
+      }
+    } else {
+      if (w * 64 < K_ITEMS) {
+        const uint8_t* p = block_of(st, w * 64 / 128);
+        const int i = tid % 128, t = i >> 2;
+        load_dwords<KD>(p + i * (KD * 4), sg.k);
+        const uint8_t* sc = p + kCodes;
+        if constexpr (FMT == IFR_KV_INT8) {
+          sg.ks[0] = reinterpret_cast<const uint16_t*>(sc)[(t & 15) * 2 + (t >> 4)];
+        } else {
+#pragma unroll
+          for (int u = 0; u < U; ++u) sg.ks[u] = reinterpret_cast<const uint32_t*>(sc)[((t & 15) * U + u) * 2 + (t >> 4)];
+        }
+      }
+      if (w * 64 < V_ITEMS) {
+        const uint8_t* p = block_of(st, w * 64 / (64 * U)) + kPart;
+        const int i = tid % (64 * U), u = i % U, gc = i / U;  // (group, c), 64 dims u
+        load_dwords<VD>(p + ((size_t)gc * N + 4 * u) * (VD), sg.v);
+        if constexpr (FMT == IFR_KV_INT8) load_dwords<4>(p + kCodes + (gc >> 4) * 16, sg.vs);
+        else load_dwords<8>(p + kCodes + ((gc >> 4) * U + u) * 32, sg.vs);
+      }
+    }
+  };
+  auto store_stage = [&](int b, int st) {
+    const int t0 = (un.p0 + NP * st) * kPgTok;
+    if (t0 < wg_lo_max || t0 + NP * kPgTok > wg_hi_min) {  // an edge step of some column
+      uint32_t bad = 0;
+      if constexpr (FMT == IFR_KV_FP16) {
+#pragma unroll
+        for (int r = 0; r < FR; ++r) {
+          const int e = tid + 256 * r;
+          uint32_t* x = reinterpret_cast<uint32_t*>(&sg.vf[r]);
+          edge_run(x, kept(t0 + 32 * (256 * r / RUNS), e % RUNS / HD, wg_lo, wg_hi), bad);
+        }
+      } else if (w * 64 < V_ITEMS) {
+        edge_scales<FMT>(sg.vs, sg.vs + 4, kept(t0 + 32 * (tid / (64 * U)), tid % (64 * U) / U >> 4, wg_lo, wg_hi), bad);
+      }
+      if (bad) aside[b] = st + 1;
+    }
+    if constexpr (FMT == IFR_KV_FP16) {
+#pragma unroll
+      for (int r = 0; r < FR; ++r) {
+        const int e = tid + 256 * r, ps = 256 * r / RUNS, i = e % RUNS;
+        lds[b][0][ps * RUNS + k_run(i >> 5, i & 31)] = sg.kf[r];
+        lds[b][1][ps * RUNS + v_run<HD>(i / HD, i % HD)] = sg.vf[r];
+      }
+    } else {
+      if (w * 64 < K_ITEMS) {
+        const int i = tid % 128, ps = tid / 128, rho = wide_row(i >> 2), g = i & 3;
+#pragma unroll
+        for (int k = 0; k < I; ++k)
+          lds[b][0][ps * RUNS + k_run(4 * k + g, rho)] = __builtin_bit_cast(
+              u4, k_values<FMT>(&sg.k[k * KD / I], sg.ks[FMT == IFR_KV_INT4 ? k / 2 : 0]));
+      }
+      if (w * 64 < V_ITEMS) {
+        const int i = tid % (64 * U), ps = tid / (64 * U), u = i % U, gc = i / U;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          lds[b][1][ps * RUNS + v_run<HD>(gc >> 4, 16 * (4 * u + n) + (gc & 15))] =
+              __builtin_bit_cast(u4, v_values<FMT>(&sg.v[n * VD / 4], sg.vs, sg.vs + 4));
+      }
+    }
+  };
+
+  // page q of the step in buffer b
+  auto page = [&](int b, int st, int q) {
+    const int t0 = (un.p0 + NP * st + q) * kPgTok;
+    if (t0 >= hi_max || t0 + kPgTok <= lo_min) return;  // (the whole wave)
+    const u4* lk = &lds[b][0][q * RUNS];
+    const u4* lv = &lds[b][1][q * RUNS];
+    v16f s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, lk[k_run(2 * k + hl, c)]), qf[k], s, 0, 0, 0);
+    const bool inner = t0 >= lo_max && t0 + kPgTok <= hi_min;
+    float x[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = s[r];
+    if (sco.mod) {
+      const float d = (float)(pos - t0 - 4 * hl);
+      modify(x, sco, a.slopes != nullptr, slope, [&](int r) { return d - (float)wide_tok(8 * (r >> 2) + (r & 3)); });
+    }
+    uint32_t seen = 0xFFFFu;
+    if (!inner) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int tk = t0 + wide_tok(8 * (r >> 2) + 4 * hl + (r & 3));
+        if (tk < lo || tk >= hi) {
+          x[r] = -INFINITY;
+          seen &= ~(1u << r);
+        }
+      }
+    }
+    float mt = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mt = fmaxf(mt, x[r]);
+    mt = fmaxf(mt, ifrd::lane_xor<32>(mt)) * sl;
+    if (!__all(!(mt > m_run + 8.0f))) {  // (as in the narrow kernel)
+      const float m_new = fmaxf(m_run, mt);
+      const float al = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= al;
+#pragma unroll
+      for (int d = 0; d < D; ++d) o[d] *= al;
+    }
+    const float mu = m_run == -INFINITY ? 0.0f : m_run;
+    v8h phi[2], plo[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(x[r], sl, -mu));
+      l_run += p;
+      const _Float16 hh = (_Float16)p;
+      phi[r >> 3][r & 7] = hh;
+      if constexpr (HL) plo[r >> 3][r & 7] = (_Float16)(p - (float)hh);
+    }
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const v8h vf = __builtin_bit_cast(v8h, lv[v_run<HD>(2 * z + hl, 32 * d + c)]);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, phi[z], o[d], 0, 0, 0);
+        if constexpr (HL) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, plo[z], o[d], 0, 0, 0);
+      }
+    if (__builtin_amdgcn_readfirstlane(aside[b]) == st + 1) {  // rare (as in the narrow kernel)
+      const uint8_t* vp = block_of(st, q) + kPart;
+#pragma unroll 1
+      for (int e = 0; e < 32; ++e) {
+        const int sb = __shfl((int)(seen >> (8 * (e >> 4) + (e & 7))) & 1, 32 * ((e >> 3) & 1) + c, 64);
+        if (!sb) continue;
+#pragma unroll 1
+        for (int k = 0; k < 16 * D; ++k)
+          ub.template add<HD, FMT>(vp, e >> 3, e & 7, 32 * (k >> 4) + 8 * ((k >> 2) & 3) + 4 * hl + (k & 3), k);
+      }
+    }
+  };
+
+  const int nst = (un.p1 - un.p0 + NP - 1) / NP;
+  if (nst > 0) {
+    load_stage(0);
+    store_stage(0, 0);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int st = 0; st < nst; ++st) {
+    const bool more = st + 1 < nst;
+    if (more) load_stage(st + 1);
+#pragma unroll 1
+    for (int q = 0; q < NP; ++q) page(st & 1, st, q);
+    if (more) store_stage((st + 1) & 1, st + 1);  // last read before the barrier of step st - 1
+    __syncthreads();
+  }
+  if (!__all(!ub.any()))
+#pragma unroll
+    for (int k = 0; k < 16 * D; ++k) o[k >> 4][k & 15] = ub.value(k, o[k >> 4][k & 15]);
+  const float l = l_run + ifrd::lane_xor<32>(l_run);
+  if (!on) return;
+  float f = 1.0f;
+  if (un.part < 0) {
+    f = l == 0.0f ? 0.0f : 1.0f / l;
+  } else if (hl == 0) {
+    float* p = a.part_ml + ((int64_t)un.part + ci) * 2;
+    p[0] = m_run;
+    p[1] = l;
+  }
+  const int64_t at = (int64_t)row * a.out_stride + (int64_t)h * HD;
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int e = 32 * d + 8 * q + 4 * hl;
+      const v4f x = (v4f){o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]} * f;
+      if (un.part >= 0)
+        *reinterpret_cast<v4f*>(a.part_o + ((int64_t)un.part + ci) * HD + e) = x;
+      else if (a.out_f32)
+        *reinterpret_cast<v4f*>(static_cast<float*>(a.out) + at + e) = x;
+      else
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at + e) =
+            make_uint2(ifrd::f2h(x[0]) | ((uint32_t)ifrd::f2h(x[1]) << 16),
+                       ifrd::f2h(x[2]) | ((uint32_t)ifrd::f2h(x[3]) << 16));
+    }
+}
+
 // ---- the splits of a column, in ascending order ------------------------------------------------
 template <int HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedJoin* joins, PagedAttnArgs a, PagedPool kv) {
@@ -526,6 +909,14 @@ hipError_t narrow_fmt(const PagedAttnArgs& a, const PagedPool& kv, int tiles, hi
   return hipGetLastError();
 }
 
+template <int HD, int FMT>
+hipError_t wide_fmt(const PagedAttnArgs& a, const PagedPool& kv, hipStream_t st) {
+  const dim3 grid(a.n_units), block(256);
+  if (a.out_f32) hipLaunchKernelGGL((paged_wide_kernel<HD, FMT, true>), grid, block, 0, st, a, kv);
+  else hipLaunchKernelGGL((paged_wide_kernel<HD, FMT, false>), grid, block, 0, st, a, kv);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 #define IFR_PAGED_DIMS(F, FMT, ...)                     \
@@ -542,20 +933,38 @@ template <int FMT>
 hipError_t paged_narrow_of(const PagedAttnArgs& a, const PagedPool& kv, int tiles, hipStream_t st) {
   IFR_PAGED_DIMS(narrow_fmt, FMT, a, kv, tiles, st);
 }
+template <int FMT>
+hipError_t paged_wide_of(const PagedAttnArgs& a, const PagedPool& kv, hipStream_t st) {
+  IFR_PAGED_DIMS(wide_fmt, FMT, a, kv, st);
+}
 template hipError_t paged_narrow_of<IFR_PAGED_FMT>(const PagedAttnArgs&, const PagedPool&, int, hipStream_t);
+template hipError_t paged_wide_of<IFR_PAGED_FMT>(const PagedAttnArgs&, const PagedPool&, hipStream_t);
 #else
 // and once without: the joins and the dispatch
 template <int FMT>
 hipError_t paged_narrow_of(const PagedAttnArgs& a, const PagedPool& kv, int tiles, hipStream_t st);
-extern template hipError_t paged_narrow_of<IFR_KV_FP16>(const PagedAttnArgs&, const PagedPool&, int, hipStream_t);
-extern template hipError_t paged_narrow_of<IFR_KV_INT8>(const PagedAttnArgs&, const PagedPool&, int, hipStream_t);
-extern template hipError_t paged_narrow_of<IFR_KV_INT4>(const PagedAttnArgs&, const PagedPool&, int, hipStream_t);
+template <int FMT>
+hipError_t paged_wide_of(const PagedAttnArgs& a, const PagedPool& kv, hipStream_t st);
+#define IFR_PAGED_EXTERN(FMT)                                                                              \
+  extern template hipError_t paged_narrow_of<FMT>(const PagedAttnArgs&, const PagedPool&, int, hipStream_t); \
+  extern template hipError_t paged_wide_of<FMT>(const PagedAttnArgs&, const PagedPool&, hipStream_t)
+IFR_PAGED_EXTERN(IFR_KV_FP16);
+IFR_PAGED_EXTERN(IFR_KV_INT8);
+IFR_PAGED_EXTERN(IFR_KV_INT4);
 
 hipError_t launch_paged_narrow(const PagedAttnArgs& a, const PagedPool& kv, int tiles, hipStream_t st) {
   if (a.n_units <= 0) return hipSuccess;
   if (kv.fmt == IFR_KV_FP16) return paged_narrow_of<IFR_KV_FP16>(a, kv, tiles, st);
   if (kv.fmt == IFR_KV_INT8) return paged_narrow_of<IFR_KV_INT8>(a, kv, tiles, st);
   if (kv.fmt == IFR_KV_INT4) return paged_narrow_of<IFR_KV_INT4>(a, kv, tiles, st);
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_paged_wide(const PagedAttnArgs& a, const PagedPool& kv, hipStream_t st) {
+  if (a.n_units <= 0) return hipSuccess;
+  if (kv.fmt == IFR_KV_FP16) return paged_wide_of<IFR_KV_FP16>(a, kv, st);
+  if (kv.fmt == IFR_KV_INT8) return paged_wide_of<IFR_KV_INT8>(a, kv, st);
+  if (kv.fmt == IFR_KV_INT4) return paged_wide_of<IFR_KV_INT4>(a, kv, st);
   return hipErrorInvalidValue;
 }
 

@@ -460,6 +460,26 @@ emu_v4f emu_mfma_f32_16x16x32_f16(emu_v8h a, emu_v8h b, emu_v4f c) {
   return d;
 }
 
+emu_v16f emu_mfma_f32_32x32x16_f16(emu_v8h a, emu_v8h b, emu_v16f c) {
+  struct P {
+    emu_v8h a, b;
+  } mine{a, b};
+  const unsigned char* s = emu::wave_exchange(&mine, sizeof(P), emu::kOpMfma);
+  const int l = emu::cur()->lane, n = l & 31, h = l >> 5;
+  _Float16 B[16];
+  for (int kb = 0; kb < 2; ++kb) std::memcpy(&B[8 * kb], s + (size_t)(n + 32 * kb) * 64 + 16, 16);
+  emu_v16f d = c;
+  for (int r = 0; r < 16; ++r) {
+    const int row = 8 * (r / 4) + 4 * h + r % 4;
+    _Float16 A[16];
+    for (int kb = 0; kb < 2; ++kb) std::memcpy(&A[8 * kb], s + (size_t)(row + 32 * kb) * 64, 16);
+    double acc = 0.0;
+    for (int k = 0; k < 16; ++k) acc += (double)(float)A[k] * (double)(float)B[k];
+    d[r] = (float)((double)c[r] + acc);
+  }
+  return d;
+}
+
 emu_v4f emu_mfma_f32_16x16x4f32(float a, float b, emu_v4f c) {
   struct P {
     float a, b;

@@ -233,6 +233,7 @@ inline unsigned emu_perm(unsigned s0, unsigned s1, unsigned sel) {
 void emu_global_load_lds(const void* g, void* l, unsigned size, int offset, int aux);
 #define __builtin_amdgcn_global_load_lds(...) emu_global_load_lds(__VA_ARGS__)
 #define __builtin_amdgcn_s_waitcnt(x) ((void)(x))
+#define __builtin_amdgcn_sched_barrier(x) ((void)(x))
 // plain loads on the host (x86 non-temporal vector loads demand alignment)
 #define __builtin_nontemporal_load(p) (*(p))
 
@@ -245,6 +246,10 @@ typedef _Float16 emu_v8h __attribute__((ext_vector_type(8)));
 // of lane l is D[4 * (l / 16) + r][l % 16].
 emu_v4i emu_mfma_i32_16x16x64_i8(emu_v4i a, emu_v4i b, emu_v4i c);
 emu_v4f emu_mfma_f32_16x16x32_f16(emu_v8h a, emu_v8h b, emu_v4f c);
+// 32x32x16: lane l holds row / column l % 32 and the K slice [8 (l / 32), +8);
+// result register r of lane l is D[8 (r / 4) + 4 (l / 32) + r % 4][l % 32].
+typedef float emu_v16f __attribute__((ext_vector_type(16)));
+emu_v16f emu_mfma_f32_32x32x16_f16(emu_v8h a, emu_v8h b, emu_v16f c);
 // (K = 4, one value per lane: k = l / 16; four fused steps in ascending k)
 emu_v4f emu_mfma_f32_16x16x4f32(float a, float b, emu_v4f c);
 inline emu_v4i emu_mfma_i8_6(emu_v4i a, emu_v4i b, emu_v4i c, int, int, int) {
@@ -253,6 +258,10 @@ inline emu_v4i emu_mfma_i8_6(emu_v4i a, emu_v4i b, emu_v4i c, int, int, int) {
 inline emu_v4f emu_mfma_f16_6(emu_v8h a, emu_v8h b, emu_v4f c, int, int, int) {
   return emu_mfma_f32_16x16x32_f16(a, b, c);
 }
+inline emu_v16f emu_mfma_f16w_6(emu_v8h a, emu_v8h b, emu_v16f c, int, int, int) {
+  return emu_mfma_f32_32x32x16_f16(a, b, c);
+}
+#define __builtin_amdgcn_mfma_f32_32x32x16_f16(...) emu_mfma_f16w_6(__VA_ARGS__)
 #define __builtin_amdgcn_mfma_i32_16x16x64_i8(...) emu_mfma_i8_6(__VA_ARGS__)
 #define __builtin_amdgcn_mfma_f32_16x16x32_f16(...) emu_mfma_f16_6(__VA_ARGS__)
 inline emu_v4f emu_mfma_f32_6(float a, float b, emu_v4f c, int, int, int) { return emu_mfma_f32_16x16x4f32(a, b, c); }

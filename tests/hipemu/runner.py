@@ -769,6 +769,22 @@ def paged_rows():
 
 
 @scenario
+def paged_chunks():
+    """A caller-owned paged cache with many rows: the workgroups that share their pages."""
+    import intfer_amd as ia
+    from tests.paged_check import run_case
+    dev, rng = ia.Device(0), np.random.default_rng(4)
+    case = lambda *a, **k: run_case(ia, dev, rng, *a, **k, say=say)  # noqa: E731
+    for fmt in (0, 1, 2):
+        case(fmt, 2, 1, 128, [70, 1], [101, 9], cap=9.0)
+        case(fmt, 1, 1, 64, [140], [300], out_f32=True)
+        case(fmt, 3, 1, 256, [12, 40], [12, 75], bias=True)
+    pos = np.arange(90, 140)
+    case(0, 1, 1, 64, [50], [140], first=np.where(pos % 5 == 0, pos + 1, pos // 40 * 40), prefix=[0])
+    case(2, 2, 1, 64, [50], [140], first=pos // 3, prefix=[130], rotary=16)
+
+
+@scenario
 def paged_refusals():
     """The calls that the paged cache refuses."""
     import intfer_amd as ia

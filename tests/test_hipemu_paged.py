@@ -7,7 +7,7 @@ import pytest
 from tests.hipemu import runner
 from tests.test_hipemu import emu_lib  # noqa: F401
 
-ORDER = ["paged_rows", "paged_refusals"]
+ORDER = ["paged_chunks", "paged_rows", "paged_refusals"]
 
 
 @pytest.fixture(scope="module")
