@@ -34,11 +34,10 @@ constexpr int64_t kMaxTokens = 1 << 30;    // tokens of a sequence
 constexpr int kKinds = 3;
 constexpr int kWidth[kKinds] = {16, 32, ifrk::kPgWide};
 
-// Units that a batch is cut into at most when there is enough of it: four
-// narrow or two wide workgroups for each of the 256 CUs; and the fewest pages
-// of a split: a page for each wave of a narrow unit, 256 tokens of a wide one.
-constexpr int64_t kUnits[kKinds] = {1024, 1024, 512};
-constexpr int kMinPages[kKinds] = {4, 4, 8};
+// The fewest pages of a split, and what a split is a multiple of: a page for
+// each wave of a narrow unit, 256 tokens of a wide one and a step's two pages.
+constexpr int kMinPages[kKinds] = {4, 4, 8}, kGrain[kKinds] = {4, 4, 2};
+constexpr int kCUs = 256;
 
 // The context's device is current while a call runs, the caller's afterwards.
 struct OnDevice {
@@ -198,17 +197,39 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
     }
     m += r;
   }
+  // Pages of a unit: the fewest for which the batch's units all run at once,
+  // so that no CU waits for a last round of few; with more tiles than that, the
+  // share of a workgroup.
   int wants[kKinds];
   for (int k = 0; k < kKinds; ++k) {
-    const int64_t per = (pages[k] * c.n_kv + kUnits[k] - 1) / kUnits[k];
-    wants[k] = (int)std::max<int64_t>(kMinPages[k], (per + 3) / 4 * 4);
+    const int64_t slots = kCUs * (k < 2 ? ifrk::paged_narrow_waves(c.format, c.head_dim, k + 1)
+                                        : ifrk::paged_wide_groups(c.head_dim));
+    const auto grain = [&](int64_t n) { return (int)std::max<int64_t>(kMinPages[k], (n + kGrain[k] - 1) / kGrain[k] * kGrain[k]); };
+    int64_t most = 0, n_tiles = 0;
+    for (const Tile& t : tiles)
+      if (t.kind == k) {
+        most = std::max<int64_t>(most, t.p1 - t.p0);
+        ++n_tiles;
+      }
+    const int64_t share = (pages[k] * c.n_kv + slots - 1) / slots;
+    int lo = grain(share), hi = std::max(lo, grain(most));
+    if (n_tiles * c.n_kv <= slots)
+      while (lo < hi) {
+        const int mid = lo + (hi - lo) / kGrain[k] / 2 * kGrain[k];
+        int64_t units = 0;
+        for (const Tile& t : tiles)
+          if (t.kind == k) units += std::max(1, (t.p1 - t.p0 + mid - 1) / mid);
+        if (units * c.n_kv <= slots) hi = mid;
+        else lo = mid + kGrain[k];
+      }
+    wants[k] = lo;
   }
   std::vector<ifrk::PagedUnit> units[kKinds];
   std::vector<ifrk::PagedJoin> joins;
   int64_t cols = 0;
   for (const Tile& t : tiles) {
     const int want = wants[t.kind], np = t.p1 - t.p0, cuts = std::max(1, (np + want - 1) / want);
-    const int step = cuts == 1 ? std::max(np, 1) : ((np + cuts - 1) / cuts + 3) / 4 * 4;
+    const int g = kGrain[t.kind], step = cuts == 1 ? std::max(np, 1) : ((np + cuts - 1) / cuts + g - 1) / g * g;
     const int ns = std::max(1, (np + step - 1) / step);
     for (int h = 0; h < c.n_kv; ++h) {
       const int64_t base = cols;
@@ -223,6 +244,10 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
           joins.push_back({row0[t.seq], h, t.col0 + i, std::min(4, t.ncol - i), (int)base + i, t.ncol, ns, 0});
     }
   }
+  // the longest first, for short ones to fill the end
+  for (auto& u : units)
+    std::stable_sort(u.begin(), u.end(),
+                     [](const ifrk::PagedUnit& x, const ifrk::PagedUnit& y) { return x.p1 - x.p0 > y.p1 - y.p0; });
   size_t at = 0;
   auto room = [&](size_t bytes) {
     const size_t o = at;

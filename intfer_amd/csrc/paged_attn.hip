@@ -279,14 +279,8 @@ __device__ __forceinline__ u4 kept(int t0, int g, int lo, int hi) {
 // 57.3 us, 16 of 32000 160.6 -> 152.3).  Bound by its VALU work at 4 bits:
 // 13 operations turn a dword of codes into 8 values.  (Two K buffers and both
 // steps unrolled spilled at 192 VGPRs: 142.8 and 467 us.)
-// (waves a SIMD: what the registers of o, q and the raw page allow)
-constexpr int narrow_waves(int fmt, int hd, int nt) {
-  if (fmt == IFR_KV_FP16 && hd >= 128) return hd == 128 ? 2 : 1;
-  return hd * nt <= 64 ? 4 : hd * nt <= 128 ? 3 : hd * nt <= 256 ? 2 : 1;
-}
-
 template <int HD, int FMT, int NT, bool HL>
-__global__ __launch_bounds__(256, narrow_waves(FMT, HD, NT)) void paged_narrow_kernel(PagedAttnArgs a, PagedPool kv) {
+__global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_narrow_kernel(PagedAttnArgs a, PagedPool kv) {
   constexpr int I = HD / 32, N = HD / 16, U = HD / kPgGroup;
   constexpr int W = FMT == IFR_KV_FP16 ? 4 : FMT == IFR_KV_INT8 ? 2 : 1;  // dwords of 8 elements
   constexpr size_t kPart = paged_part(FMT, HD);
@@ -591,7 +585,7 @@ template <int HD>
 __device__ __forceinline__ int v_run(int g, int d) { return g * HD + (d ^ ((d >> 4) & 15)); }
 
 template <int HD, int FMT, bool HL>
-__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_wide_kernel(PagedAttnArgs a, PagedPool kv) {
+__global__ __launch_bounds__(256, paged_wide_groups(HD)) void paged_wide_kernel(PagedAttnArgs a, PagedPool kv) {
   constexpr int NP = HD == 256 ? 1 : 2;
   constexpr int I = HD / 32, N = HD / 16, U = HD / kPgGroup, KS = HD / 16, D = HD / 32;
   constexpr int RUNS = 4 * HD;  // 16-byte runs of a page's K (or V) in LDS
