@@ -71,8 +71,8 @@ struct PagedUnit {
   int p0, p1;
   int part;   // first partial column, or -1: the unit writes the output itself
 };
-// Partials of columns [col0, col0 + n): split s of column i is partial column
-// base + s * stride + i.
+// Partials of columns [col0, col0 + n), at most 1024 / hd of them: split s of
+// column i is partial column base + s * stride + i.
 struct PagedJoin {
   int row0, kvh, col0, n, base, stride, ns, pad;
 };

@@ -240,8 +240,8 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
       }
       if (cols > kMaxTokens) return fail(IFR_EINVAL, "too many partial columns");
       if (ns > 1)
-        for (int i = 0; i < t.ncol; i += 4)
-          joins.push_back({row0[t.seq], h, t.col0 + i, std::min(4, t.ncol - i), (int)base + i, t.ncol, ns, 0});
+        for (int i = 0, n = 1024 / c.head_dim; i < t.ncol; i += n)
+          joins.push_back({row0[t.seq], h, t.col0 + i, std::min(n, t.ncol - i), (int)base + i, t.ncol, ns, 0});
     }
   }
   // the longest first, for short ones to fill the end

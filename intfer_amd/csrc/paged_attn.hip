@@ -120,11 +120,12 @@ __device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t* w) {
 // keep their bits.  While every |a / cap| of the wave is at most 1/2 (scores
 // hardly ever come near their cap) it is x P(x^2), P the degree-4 Chebyshev
 // interpolation of tanh(x) / x in x^2 on [0, 1/4] (1.4e-8 off), 7 operations a
-// score; else 1 - 2 / (e^2x + 1) above 1/2.  The bias takes |pos - t| in fp32,
+// score with the factors inside; else 1 - 2 / (e^2x + 1) above 1/2.  The bias takes |pos - t| in fp32,
 // exact up to 2^24; far(j) is pos - t of score j.
 struct Scoring {
   float scale2;           // scale log2 e
   float inv, cap2;        // scale / cap, cap log2 e; inv 0: no cap
+  float c[5];             // cap2 P
   bool mod;               // cap or bias
 };
 __device__ __forceinline__ Scoring scoring(const PagedAttnArgs& a) {
@@ -132,6 +133,11 @@ __device__ __forceinline__ Scoring scoring(const PagedAttnArgs& a) {
   s.scale2 = a.scale * kLog2e;
   s.inv = a.cap != 0.0f ? a.scale / a.cap : 0.0f;
   s.cap2 = a.cap * kLog2e;
+  s.c[0] = 0.99999999f * s.cap2;
+  s.c[1] = -0.333330679f * s.cap2;
+  s.c[2] = 0.133247505f * s.cap2;
+  s.c[3] = -0.0529842388f * s.cap2;
+  s.c[4] = 0.0171313444f * s.cap2;
   s.mod = a.cap != 0.0f || a.slopes != nullptr;
   return s;
 }
@@ -144,19 +150,19 @@ __device__ __forceinline__ void modify(float (&x)[C], const Scoring& s, bool bia
       x[j] *= s.inv;
       big = fmaxf(big, fabsf(x[j]));
     }
-    auto poly = [](float v) {
+    auto poly = [&](float v) {
       const float y = v * v;
-      return v * fmaf(fmaf(fmaf(fmaf(0.0171313444f, y, -0.0529842388f), y, 0.133247505f), y, -0.333330679f), y, 0.99999999f);
+      return v * fmaf(fmaf(fmaf(fmaf(s.c[4], y, s.c[3]), y, s.c[2]), y, s.c[1]), y, s.c[0]);
     };
     if (__all(!(big > 0.5f))) {
 #pragma unroll
-      for (int j = 0; j < C; ++j) x[j] = poly(x[j]) * s.cap2;
+      for (int j = 0; j < C; ++j) x[j] = poly(x[j]);
     } else {
 #pragma unroll
       for (int j = 0; j < C; ++j) {
         const float e = __builtin_amdgcn_exp2f(fabsf(x[j]) * (2.0f * kLog2e));
         const float t = __builtin_copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f), x[j]);
-        x[j] = (fabsf(x[j]) > 0.5f ? t : poly(x[j])) * s.cap2;
+        x[j] = fabsf(x[j]) > 0.5f ? t * s.cap2 : poly(x[j]);
         __builtin_amdgcn_sched_barrier(0);  // (one at a time: the seldom case is to hold few registers)
       }
     }
@@ -267,6 +273,58 @@ __device__ __forceinline__ u4 kept(int t0, int g, int lo, int hi) {
   }
   return keep;
 }
+// ---- the splits of a column, in ascending order ------------------------------------------------
+// HD / 4 lanes a column, 4 dims each: a wave takes 256 / HD columns (a wave a
+// column read 4 bytes a lane: 32000 columns of 64 dims 16.4 us).  A launch of
+// its own: a unit that finds itself the last of its tile and joins in place needs
+// the device's L2 caches written back and dropped by every unit, which made 64
+// rows of 2048 int4 tokens 116 us instead of 43.
+template <int HD>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedJoin* joins, PagedAttnArgs a, PagedPool kv) {
+  constexpr int LPC = HD / 4;
+  const PagedJoin j = joins[blockIdx.x];
+  const int i = threadIdx.x / LPC, d = (threadIdx.x % LPC) * 4;
+  if (i >= j.n) return;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
+  const int64_t base = (int64_t)j.base + i;
+  float m = -INFINITY, l = 0.0f;
+  v4f x = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < j.ns; s0 += 8) {
+    float2 q[8];
+    v4f p[8];
+    float mr = m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {  // (clamped, unconditional: one latency a round)
+      const int64_t e = base + (int64_t)min(s0 + k, j.ns - 1) * j.stride;
+      q[k] = ml[e];
+      p[k] = *reinterpret_cast<const v4f*>(a.part_o + e * HD + d);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mr = fmaxf(mr, q[k].x);
+    const float mu = mr == -INFINITY ? 0.0f : mr;
+    const float al = __builtin_amdgcn_exp2f(m - mu);
+    l *= al;
+    x *= al;
+    m = mr;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (s0 + k >= j.ns || q[k].x == -INFINITY) continue;
+      const float f = __builtin_amdgcn_exp2f(q[k].x - mu);
+      l += f * q[k].y;
+      x += p[k] * f;
+    }
+  }
+  x *= l == 0.0f ? 0.0f : 1.0f / l;
+  const int G = kv.nq / kv.nkv, col = j.col0 + i;
+  const int64_t at = (int64_t)(j.row0 + col / G) * a.out_stride + (int64_t)(j.kvh * G + col % G) * HD + d;
+  if (a.out_f32)
+    *reinterpret_cast<v4f*>(static_cast<float*>(a.out) + at) = x;
+  else
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
+        make_uint2(ifrd::f2h(x[0]) | ((uint32_t)ifrd::f2h(x[1]) << 16),
+                   ifrd::f2h(x[2]) | ((uint32_t)ifrd::f2h(x[3]) << 16));
+}
+
 // ---- few columns: the four waves of a workgroup take every fourth page ------------------------
 //
 // A wave holds NT tiles of 16 columns.  The next page's K is loaded once the
@@ -845,51 +903,6 @@ __global__ __launch_bounds__(256, paged_wide_groups(HD)) void paged_wide_kernel(
             make_uint2(ifrd::f2h(x[0]) | ((uint32_t)ifrd::f2h(x[1]) << 16),
                        ifrd::f2h(x[2]) | ((uint32_t)ifrd::f2h(x[3]) << 16));
     }
-}
-
-// ---- the splits of a column, in ascending order ------------------------------------------------
-template <int HD>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedJoin* joins, PagedAttnArgs a, PagedPool kv) {
-  constexpr int E = HD / 64;  // dims of a lane
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const PagedJoin j = joins[blockIdx.x];
-  if (w >= j.n) return;
-  const int G = kv.nq / kv.nkv;
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
-  const int64_t base = (int64_t)j.base + w;
-  float m = -INFINITY;
-  for (int s = 0; s < j.ns; ++s) m = fmaxf(m, ml[base + (int64_t)s * j.stride].x);
-  const float mu = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, x[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) x[e] = 0.0f;
-  for (int s0 = 0; s0 < j.ns; s0 += 8) {
-    float2 q[8];
-    float p[8][E];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {  // (clamped, unconditional: one latency a round)
-      const int64_t i = base + (int64_t)min(s0 + k, j.ns - 1) * j.stride;
-      q[k] = ml[i];
-#pragma unroll
-      for (int e = 0; e < E; ++e) p[k][e] = a.part_o[i * HD + lane * E + e];
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (s0 + k >= j.ns || q[k].x == -INFINITY) continue;
-      const float f = __builtin_amdgcn_exp2f(q[k].x - mu);
-      l += f * q[k].y;
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] += f * p[k][e];
-    }
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const int col = j.col0 + w;
-  const int64_t at = (int64_t)(j.row0 + col / G) * a.out_stride + (int64_t)(j.kvh * G + col % G) * HD + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (a.out_f32) static_cast<float*>(a.out)[at + e] = x[e] * inv;
-    else static_cast<uint16_t*>(a.out)[at + e] = ifrd::f2h(x[e] * inv);
-  }
 }
 
 template <int HD, int FMT>

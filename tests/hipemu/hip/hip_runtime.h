@@ -141,7 +141,6 @@ void note_queued(hipStream_t st);  // work went onto st (until the stream is wai
 }
 
 inline void __syncthreads() { emu::block_barrier(); }
-
 // ---- cross-lane builtins ---------------------------------------------------------
 namespace emu {
 enum { kOpShfl = 1, kOpDpp = 2, kOpReadlane = 3, kOpFirst = 4, kOpMfma = 5 };
