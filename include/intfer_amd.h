@@ -370,7 +370,7 @@ int ifr_paged_set(ifr_paged* p, const ifr_paged_batch* b);
  * back to back inside a row; 16-byte aligned, strides a multiple of 8 (slices
  * of a fused QKV output qualify).  The rotation is rotate-half (rope,
  * main.cpp:365-373) over the first `rotary` dims with the fp32 tables
- * cos_d, sin_d [max_pos][rotary / 2], in fp32; K is stored from the fp32
+ * cos_d, sin_d [max_pos][rotary / 2] (16-byte aligned), in fp32; K is stored from the fp32
  * result.  Q is rotated into q_out_d, which is q_d itself (same stride) or
  * overlaps nothing; both NULL: no Q. */
 typedef struct ifr_paged_rows {

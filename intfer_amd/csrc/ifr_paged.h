@@ -58,8 +58,8 @@ struct PagedPool {
 struct PagedRow {       // one row of the batch: it sees positions [lo, hi)
   int lo, hi, pos, seq;
 };
-struct PagedRun {       // rows [row, row + n) are tokens [t0, t0 + n) of a page
-  int page, t0, n, row;
+struct PagedRun {       // rows [row, row + n) are tokens [t0, t0 + n) of a page, positions from pos
+  int page, t0, n, row, pos, pad[3];
 };
 // One workgroup of attention: columns [col0, col0 + ncol) of a sequence (column
 // = new row * G + head of the kv head's group) over its pages [p0, p1).

@@ -173,7 +173,7 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
       const int t0 = pos % kPgTok, k = std::min(kPgTok - t0, n - pos), pg = t[pos / kPgTok];
       if (written[pg]) appendable = false;
       written[pg] = 1;
-      runs.push_back({pg, t0, k, (int)(m + pos - (n - r))});
+      runs.push_back({pg, t0, k, (int)(m + pos - (n - r)), pos, {0, 0, 0}});
       pos += k;
     }
     const int64_t ncols = (int64_t)r * G;
@@ -400,7 +400,8 @@ int ifr_paged_append(ifr_paged* p, void* pool_d, const ifr_paged_rows* r) {
   if (int e = rows_ok("k_d", r->k_d, r->k_stride, kw, 2)) return e;
   if (int e = rows_ok("v_d", r->v_d, r->v_stride, kw, 2)) return e;
   if (!r->q_d != !r->q_out_d) return fail(IFR_EINVAL, "q_d and q_out_d go together");
-  if (r->rotary && (!r->cos_d || !r->sin_d)) return fail(IFR_EINVAL, "rotary %d without its tables", r->rotary);
+  if (r->rotary && (!r->cos_d || !r->sin_d || !aligned(r->cos_d, 16) || !aligned(r->sin_d, 16)))
+    return fail(IFR_EINVAL, "rotary %d: its tables are null or not on 16 bytes", r->rotary);
   if (r->rotary && p->max_pos >= r->max_pos)
     return fail(IFR_EINVAL, "position %d, tables of %d positions", p->max_pos, r->max_pos);
   const int64_t pb = (int64_t)pool_bytes(c);

@@ -20,10 +20,7 @@ namespace ifrk {
 namespace {
 
 constexpr float kMaxHalf = 65504.0f;
-
-__device__ __forceinline__ bool finite_f(float x) {
-  return (__builtin_bit_cast(uint32_t, x) & 0x7F800000u) != 0x7F800000u;
-}
+constexpr int kHalfMirror = 0x141;  // DPP: lane i of 8 reads lane 7 - i
 
 // Reductions over the 8, 16 or 32 consecutive lanes that share a token (all
 // lanes of the wave take part).
@@ -31,36 +28,43 @@ template <int LPT>
 __device__ __forceinline__ float group_max(float v) {
   v = fmaxf(v, ifrd::lane_xor<1>(v));
   v = fmaxf(v, ifrd::lane_xor<2>(v));
-  v = fmaxf(v, ifrd::lane_xor<4>(v));
+  v = fmaxf(v, ifrd::dpp_f<kHalfMirror>(v));  // (the quads are uniform: any lane of the other one)
   if constexpr (LPT >= 16) v = fmaxf(v, ifrd::lane_xor<8>(v));
   if constexpr (LPT >= 32) v = fmaxf(v, ifrd::lane_xor<16>(v));
   return v;
 }
+// Whether one of the lanes' values is a NaN or an infinity (0 x is 0 of none else).
+template <int LPT>
+__device__ __forceinline__ bool group_bad(const float (&x)[8]) {
+  float t = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t = fmaf(x[e], 0.0f, t);
+  constexpr uint64_t kLanes = LPT >= 32 ? 0xFFFFFFFFull : (1ull << LPT) - 1;
+  return (__ballot(t != t) >> (threadIdx.x & 63 & ~(LPT - 1)) & kLanes) != 0;
+}
 
 // Quantize a lane's 8 consecutive dims.  int8: the scale of the whole head row
-// (LPT lanes); int4: of its 64 dims (8 lanes).  Codes as bytes.
-template <int FMT, int LPT>
+// (LPT lanes); int4: of its 64 dims (8 lanes).  Codes as bytes or, NIBBLES, as
+// the int4 dword of 8 elements.
+template <int FMT, int LPT, bool NIBBLES>
 __device__ __forceinline__ void quantize8(const float (&x)[8], uint32_t (&code)[2], uint16_t& scale, uint16_t& zero) {
-  code[0] = code[1] = 0u;
-  float bad = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (!finite_f(x[e])) bad = 1.0f;
   if constexpr (FMT == IFR_KV_INT8) {
+    const bool bad = group_bad<LPT>(x);
     float a = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(x[e]));
     a = group_max<LPT>(a);
-    bad = group_max<LPT>(bad);
-    scale = bad != 0.0f ? (uint16_t)0x7E00u : ifrd::f2h(fminf(a / 127.0f, 515.5f));
+    scale = bad ? (uint16_t)0x7E00u : ifrd::f2h(fminf(a / 127.0f, 515.5f));
     const float s = ifrd::h2f(scale);
-    const float inv = s > 0.0f && bad == 0.0f ? 1.0f / s : 0.0f;
+    const float inv = s > 0.0f && !bad ? 1.0f / s : 0.0f;
+    code[0] = code[1] = 0u;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float v = bad != 0.0f ? 0.0f : x[e];
+      const float v = bad ? 0.0f : x[e];
       code[e >> 2] |= ((uint32_t)ifrd::quant_half_away(v, inv) & 0xFFu) << (8 * (e & 3));
     }
   } else if constexpr (FMT == IFR_KV_INT4) {
+    const bool bad = group_bad<8>(x);
     float hi = -INFINITY, lo = INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -69,23 +73,30 @@ __device__ __forceinline__ void quantize8(const float (&x)[8], uint32_t (&code)[
     }
     hi = group_max<8>(hi);
     lo = -group_max<8>(-lo);
-    bad = group_max<8>(bad);
     lo = fminf(fmaxf(lo, -kMaxHalf), kMaxHalf);  // (a rotated value can pass fp16's range)
     hi = fminf(fmaxf(hi, -kMaxHalf), kMaxHalf);
     scale = ifrd::f2h((hi - lo) / 15.0f);
     zero = ifrd::f2h(lo);
     if (15.0f * ifrd::h2f(scale) + ifrd::h2f(zero) >= 65520.0f) scale -= 1;  // code 15 would round to infinity
-    if (bad != 0.0f) {
+    if (bad) {
       scale = 0x7E00u;
       zero = 0u;
     }
     const float s = ifrd::h2f(scale), z = ifrd::h2f(zero);
-    const float inv = s > 0.0f && bad == 0.0f ? 1.0f / s : 0.0f;
+    const float inv = s > 0.0f && !bad ? 1.0f / s : 0.0f;
+    float c[8];  // (the clamp also turns the NaN of a bad group's infinity times zero into a code)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = bad != 0.0f ? 0.0f : (x[e] - z) * inv;
-      const int c = (int)fminf(fmaxf(__builtin_rintf(v), 0.0f), 15.0f);
-      code[e >> 2] |= (uint32_t)c << (8 * (e & 3));
+    for (int e = 0; e < 8; ++e) c[e] = fminf(fmaxf(__builtin_rintf((x[e] - z) * inv), 0.0f), 15.0f);
+    // codes side by side by exact fp32 sums: 16 bits at a time
+    if constexpr (NIBBLES) {
+      const float even = fmaf(c[6], 4096.0f, fmaf(c[4], 256.0f, fmaf(c[2], 16.0f, c[0])));
+      const float odd = fmaf(c[7], 4096.0f, fmaf(c[5], 256.0f, fmaf(c[3], 16.0f, c[1])));
+      code[0] = (uint32_t)even | ((uint32_t)odd << 16);
+      code[1] = 0u;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        code[q] = (uint32_t)fmaf(c[4 * q + 1], 256.0f, c[4 * q]) | ((uint32_t)fmaf(c[4 * q + 3], 256.0f, c[4 * q + 2]) << 16);
     }
   }
 }
@@ -102,86 +113,96 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Bytes of codes -> the int4 dword of 8 elements.
-__device__ __forceinline__ uint32_t pack_nibbles(const uint32_t (&b)[2]) {
-  uint32_t w = 0;
+// 8 values of a rotation table (16-byte aligned rows: half is a multiple of 8)
+__device__ __forceinline__ void load_table(const float* p, float (&x)[8]) {
+  const v4f u = reinterpret_cast<const v4f*>(p)[0], v = reinterpret_cast<const v4f*>(p)[1];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w |= ((b[e >> 2] >> (8 * (e & 3))) & 15u) << (4 * paged_nibble(e));
-  return w;
+  for (int e = 0; e < 4; ++e) {
+    x[e] = u[e];
+    x[4 + e] = v[e];
+  }
 }
 
-// One wave per (run, kv head): up to 32 tokens of one page.  HD / 8 lanes hold
-// a token, 8 dims each.  K goes straight to its place; V, whose 8-element runs
-// are 8 tokens of one dim, crosses through LDS.  A run of V that the tokens
-// cover whole is stored whole, else element by element (fp16, int8) or as a
-// read-modify-write of its dword (int4; a batch writes a page from one run
-// only, so nobody else has that dword).  The blocks past the runs rotate Q.
+// Rows a workgroup rotates of Q, about four items a thread.
+__host__ __device__ inline int q_rows(int items) { return items >= 1024 ? 1 : 1024 / items; }
+
+// One workgroup per (run, kv head): up to 32 tokens of one page.  HD / 8 lanes
+// hold a token, 8 dims each, so 2048 / HD tokens are in hand at once and a page
+// is one to four such passes (loading all of them ahead took 126 registers at
+// 256 dims and left the blocks that rotate Q three waves a SIMD).  K goes
+// straight to its place; V, whose 8-element runs are 8 tokens of one dim, crosses
+// through LDS.  A run of V that the tokens cover whole is stored whole, else
+// element by element (fp16, int8) or as a read-modify-write of its dword (int4; a
+// batch writes a page from one run only, so nobody else has that dword).  The
+// blocks past the runs rotate Q.
 template <int HD, int FMT>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, PagedPool kv, int kv_blocks) {
-  constexpr int LPT = HD / 8, TPI = 64 / LPT, U = HD / kPgGroup;
+  constexpr int LPT = HD / 8, TP = 256 / LPT, PASSES = kPgTok / TP, U = HD / kPgGroup;
   constexpr int ES = FMT == IFR_KV_FP16 ? 2 : 1;   // bytes of an element in LDS
   constexpr int LROW = HD * ES + 16;
-  __shared__ __align__(16) uint8_t stage[4][kPgTok * LROW];
-  const int half = a.r.rotary / 2;
+  __shared__ __align__(16) uint8_t st[kPgTok * LROW];
+  const int half = a.r.rotary / 2, tid = threadIdx.x;
   if ((int)blockIdx.x >= kv_blocks) {
     // Q: an item is 8 dims and their partners, or 8 dims past the rotation
-    const int np = half / 8, ni = np + (HD - a.r.rotary) / 8;
-    const int64_t item = ((int64_t)blockIdx.x - kv_blocks) * 256 + threadIdx.x;
-    if (item >= (int64_t)a.M * kv.nq * ni) return;
-    const int p = (int)(item % ni);
-    const int64_t mh = item / ni;
-    const int h = (int)(mh % kv.nq), m = (int)(mh / kv.nq);
-    const uint16_t* src = a.r.q_d + (int64_t)m * a.r.q_stride + (int64_t)h * HD;
-    uint16_t* dst = a.r.q_out_d + (int64_t)m * a.r.q_out_stride + (int64_t)h * HD;
-    if (p >= np) {
-      const int d = a.r.rotary + 8 * (p - np);
-      *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(src + d);
-      return;
-    }
-    const int64_t t = (int64_t)a.rows[m].pos * half + 8 * p;
-    float x[8], y[8], u[8], v[8];
-    load8(src + 8 * p, x);
-    load8(src + half + 8 * p, y);
+    const unsigned np = half / 8, ni = np + (HD - a.r.rotary) / 8, per = ni * kv.nq, nr = q_rows((int)per);
+    const int m0 = ((int)blockIdx.x - kv_blocks) * (int)nr;
+    const unsigned n = min((int)nr, a.M - m0) * per;
+    for (unsigned i = tid; i < n; i += 256) {
+      const unsigned r = i / per, hp = i - r * per, h = hp / ni, p = hp - h * ni;
+      const int m = m0 + (int)r;
+      const uint16_t* src = a.r.q_d + (int64_t)m * a.r.q_stride + (int64_t)h * HD;
+      uint16_t* dst = a.r.q_out_d + (int64_t)m * a.r.q_out_stride + (int64_t)h * HD;
+      if (p >= np) {
+        const int d = a.r.rotary + 8 * (int)(p - np);
+        *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(src + d);
+        continue;
+      }
+      const int64_t t = (int64_t)a.rows[m].pos * half + 8 * p;
+      float x[8], y[8], c[8], s[8], u[8], v[8];
+      load8(src + 8 * p, x);
+      load8(src + half + 8 * p, y);
+      load_table(a.r.cos_d + t, c);
+      load_table(a.r.sin_d + t, s);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float c = a.r.cos_d[t + e], s = a.r.sin_d[t + e];
-      u[e] = x[e] * c - y[e] * s;
-      v[e] = y[e] * c + x[e] * s;
+      for (int e = 0; e < 8; ++e) {
+        u[e] = x[e] * c[e] - y[e] * s[e];
+        v[e] = y[e] * c[e] + x[e] * s[e];
+      }
+      *reinterpret_cast<uint4*>(dst + 8 * p) = pack8(u);
+      *reinterpret_cast<uint4*>(dst + half + 8 * p) = pack8(v);
     }
-    *reinterpret_cast<uint4*>(dst + 8 * p) = pack8(u);
-    *reinterpret_cast<uint4*>(dst + half + 8 * p) = pack8(v);
     return;
   }
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t item = (int64_t)blockIdx.x * 4 + w;
-  if (item >= (int64_t)a.n_runs * kv.nkv) return;
-  const PagedRun run = a.runs[item / kv.nkv];
-  const int kvh = (int)(item % kv.nkv);
+  const unsigned item = blockIdx.x, ri = item / (unsigned)kv.nkv;
+  const PagedRun run = a.runs[ri];
+  const int kvh = (int)(item - ri * kv.nkv);
   uint8_t* kpart = kv.pool + (size_t)run.page * paged_page(FMT, HD, kv.nkv) + (size_t)kvh * 2 * paged_part(FMT, HD);
   uint8_t* vpart = kpart + paged_part(FMT, HD);
   constexpr size_t codes = FMT == IFR_KV_FP16 ? 0 : FMT == IFR_KV_INT8 ? 32 * HD : 16 * HD;
   uint16_t* kscale = reinterpret_cast<uint16_t*>(kpart + codes);
   uint16_t* vscale = reinterpret_cast<uint16_t*>(vpart + codes);
-  uint8_t* st = stage[w];
-  const int sub = lane / LPT, d0 = (lane % LPT) * 8, u = d0 / kPgGroup;
-  for (int b = 0; b < run.n; b += TPI) {
-    const int i = b + sub, t = run.t0 + i;
+  const int sub = tid / LPT, d0 = (tid % LPT) * 8, u = d0 / kPgGroup;
+  const bool turns = d0 < a.r.rotary;
+  const int ds = d0 < half ? d0 : d0 - half;  // where the pair's table values are
+#pragma unroll 1
+  for (int q = 0; q < PASSES; ++q) {
+    if (q * TP >= run.n) break;
+    const int i = q * TP + sub, t = run.t0 + i;
     const bool on = i < run.n;
     const int64_t m = run.row + (on ? i : 0);
     const uint16_t* kr = a.r.k_d + m * a.r.k_stride + (int64_t)kvh * HD;
-    const uint16_t* vr = a.r.v_d + m * a.r.v_stride + (int64_t)kvh * HD;
     float x[8], y[8];
     load8(kr + d0, x);
-    load8(vr + d0, y);
-    if (d0 < a.r.rotary) {
-      const int ds = d0 < half ? d0 : d0 - half;
-      float p[8];
+    load8(a.r.v_d + m * a.r.v_stride + (int64_t)kvh * HD + d0, y);
+    if (turns) {
+      float p[8], c[8], s[8];
       load8(kr + (d0 < half ? d0 + half : ds), p);
-      const int64_t tb = (int64_t)a.rows[m].pos * half + ds;
+      const int64_t tb = (int64_t)(run.pos + (on ? i : 0)) * half + ds;
+      load_table(a.r.cos_d + tb, c);
+      load_table(a.r.sin_d + tb, s);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float c = a.r.cos_d[tb + e], s = a.r.sin_d[tb + e];
-        const float xc = x[e] * c, ps = p[e] * s;
+        const float xc = x[e] * c[e], ps = p[e] * s[e];
         x[e] = d0 < half ? xc - ps : xc + ps;
       }
     }
@@ -193,8 +214,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, Pa
     } else {
       uint32_t kc[2], vc[2];
       uint16_t ks, kz, vs, vz;
-      quantize8<FMT, LPT>(x, kc, ks, kz);
-      quantize8<FMT, LPT>(y, vc, vs, vz);
+      quantize8<FMT, LPT, FMT == IFR_KV_INT4>(x, kc, ks, kz);
+      quantize8<FMT, LPT, false>(y, vc, vs, vz);
       if (on) {
         *reinterpret_cast<uint2*>(st + t * LROW + d0) = make_uint2(vc[0], vc[1]);
         if constexpr (FMT == IFR_KV_INT8) {
@@ -204,7 +225,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, Pa
             vscale[paged_vscale(FMT, HD, t, 0)] = vs;
           }
         } else {
-          *reinterpret_cast<uint32_t*>(kpart + paged_koff(FMT, HD, t, d0) / 2) = pack_nibbles(kc);
+          *reinterpret_cast<uint32_t*>(kpart + paged_koff(FMT, HD, t, d0) / 2) = kc[0];
           if (d0 % kPgGroup == 0) {
             *reinterpret_cast<uint32_t*>(kscale + paged_kscale(FMT, HD, t, u)) = (uint32_t)ks | ((uint32_t)kz << 16);
             vscale[paged_vscale(FMT, HD, t, u)] = vs;
@@ -214,40 +235,47 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, Pa
       }
     }
   }
-  ifrd::wave_sync();
+  __syncthreads();
   const int t1 = run.t0 + run.n;
-  // run r of 8 tokens: group g, dim d; only groups that hold a token of ours
-  for (int r = lane; r < 4 * HD; r += 64) {
-    const int g = r / HD;
-    const int d = FMT == IFR_KV_FP16 ? r % HD : (r % (HD / 16)) * 16 + (r % HD) / (HD / 16);
-    uint32_t mine = 0;
+  // A thread takes 4 bytes of each of a group's 8 tokens, 2 or 4 dims, and turns
+  // them into those dims' runs; only groups that hold a token of ours.
+  constexpr int DPI = 4 / ES;
+  for (int i = tid; i < 4 * HD / DPI; i += 256) {
+    const int g = i / (HD / DPI), d = i % (HD / DPI) * DPI;
+    uint32_t mine = 0, w[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int t = paged_vtok(g, j);
-      if (t >= run.t0 && t < t1) mine |= 1u << j;
+      const bool in = t >= run.t0 && t < t1;
+      mine |= (uint32_t)in << j;
+      w[j] = in ? *reinterpret_cast<const uint32_t*>(st + t * LROW + d * ES) : 0u;
     }
     if (!mine) continue;
     if constexpr (FMT == IFR_KV_FP16) {
-      uint16_t x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = (mine >> j) & 1 ? *reinterpret_cast<const uint16_t*>(st + paged_vtok(g, j) * LROW + d * 2) : 0;
-      uint16_t* dst = reinterpret_cast<uint16_t*>(vpart) + (size_t)r * 8;
-      if (mine == 0xFFu) {
-        *reinterpret_cast<uint4*>(dst) =
-            make_uint4(x[0] | ((uint32_t)x[1] << 16), x[2] | ((uint32_t)x[3] << 16), x[4] | ((uint32_t)x[5] << 16),
-                       x[6] | ((uint32_t)x[7] << 16));
-      } else {
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t sel = e ? 0x07060302u : 0x05040100u;  // the e-th halves of two dwords
+        uint16_t* dst = reinterpret_cast<uint16_t*>(vpart) + (size_t)(g * HD + d + e) * 8;
+        uint32_t x[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if ((mine >> j) & 1) dst[j] = x[j];
+        for (int j = 0; j < 4; ++j) x[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], sel);
+        if (mine == 0xFFu) {
+          *reinterpret_cast<uint4*>(dst) = make_uint4(x[0], x[1], x[2], x[3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if ((mine >> j) & 1) dst[j] = (uint16_t)(x[j >> 1] >> (16 * (j & 1)));
+        }
       }
-    } else {
-      uint32_t x[2] = {0u, 0u};
+    } else if constexpr (FMT == IFR_KV_INT8) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if ((mine >> j) & 1) x[j >> 2] |= (uint32_t)st[paged_vtok(g, j) * LROW + d] << (8 * (j & 3));
-      if constexpr (FMT == IFR_KV_INT8) {
-        uint8_t* dst = vpart + (size_t)r * 8;
+      for (int e = 0; e < 4; ++e) {
+        uint8_t* dst = vpart + (size_t)paged_vrun(FMT, HD, g, d + e) * 8;
+        const uint32_t sel = 0x0C0C0400u + e * 0x0101u;  // byte e of two dwords
+        uint32_t x[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          x[q] = __builtin_amdgcn_perm(w[4 * q + 1], w[4 * q], sel) | (__builtin_amdgcn_perm(w[4 * q + 3], w[4 * q + 2], sel) << 16);
         if (mine == 0xFFu) {
           *reinterpret_cast<uint2*>(dst) = make_uint2(x[0], x[1]);
         } else {
@@ -255,13 +283,19 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, Pa
           for (int j = 0; j < 8; ++j)
             if ((mine >> j) & 1) dst[j] = (uint8_t)(x[j >> 2] >> (8 * (j & 3)));
         }
-      } else {
-        uint32_t* dst = reinterpret_cast<uint32_t*>(vpart) + r;
-        uint32_t keep = 0;
+      }
+    } else {
+      // even tokens' nibbles side by side, then odd ones' (paged_nibble)
+      const uint32_t p = w[0] | (w[2] << 4), q = w[4] | (w[6] << 4), r = w[1] | (w[3] << 4), u2 = w[5] | (w[7] << 4);
+      uint32_t keep = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (!((mine >> j) & 1)) keep |= 15u << (4 * paged_nibble(j));
-        const uint32_t nw = pack_nibbles(x);
+      for (int j = 0; j < 8; ++j)
+        if (!((mine >> j) & 1)) keep |= 15u << (4 * paged_nibble(j));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t* dst = reinterpret_cast<uint32_t*>(vpart) + paged_vrun(FMT, HD, g, d + e);
+        const uint32_t sel = 0x0C0C0400u + e * 0x0101u;
+        const uint32_t nw = __builtin_amdgcn_perm(q, p, sel) | (__builtin_amdgcn_perm(u2, r, sel) << 16);
         *dst = keep ? (*dst & keep) | nw : nw;
       }
     }
@@ -280,81 +314,91 @@ __device__ __forceinline__ uint16_t value_of(int c, uint16_t s, uint16_t z) {
   }
 }
 
-// One wave per (run, kv head): the inverse of the append, into [M][nkv][HD].
-// Whole 8-token runs of V are read (they are inside the page), the tokens of
-// the run are written.
+// One workgroup per (run, kv head): the inverse of the append, into
+// [M][nkv][HD].  Whole 8-token runs of V are read (they are inside the page), the
+// tokens of the run are written.
 template <int HD, int FMT>
-__global__ __launch_bounds__(256) void paged_read_kernel(const PagedRun* runs, int n_runs, uint16_t* k, uint16_t* v,
-                                                         PagedPool kv) {
-  constexpr int LPT = HD / 8, TPI = 64 / LPT;
+__global__ __launch_bounds__(256) void paged_read_kernel(const PagedRun* runs, uint16_t* k, uint16_t* v, PagedPool kv) {
+  constexpr int LPT = HD / 8, TP = 256 / LPT, PASSES = kPgTok / TP, VR = HD / 64;
   constexpr int LROW = HD * 2 + 16;
-  __shared__ __align__(16) uint8_t stage[4][kPgTok * LROW];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t item = (int64_t)blockIdx.x * 4 + w;
-  if (item >= (int64_t)n_runs * kv.nkv) return;
-  const PagedRun run = runs[item / kv.nkv];
-  const int kvh = (int)(item % kv.nkv);
+  __shared__ __align__(16) uint8_t st[kPgTok * LROW];
+  const int tid = threadIdx.x;
+  const unsigned item = blockIdx.x, ri = item / (unsigned)kv.nkv;
+  const PagedRun run = runs[ri];
+  const int kvh = (int)(item - ri * kv.nkv);
   const uint8_t* kpart =
       kv.pool + (size_t)run.page * paged_page(FMT, HD, kv.nkv) + (size_t)kvh * 2 * paged_part(FMT, HD);
   const uint8_t* vpart = kpart + paged_part(FMT, HD);
   constexpr size_t codes = FMT == IFR_KV_FP16 ? 0 : FMT == IFR_KV_INT8 ? 32 * HD : 16 * HD;
   const uint16_t* kscale = reinterpret_cast<const uint16_t*>(kpart + codes);
   const uint16_t* vscale = reinterpret_cast<const uint16_t*>(vpart + codes);
-  uint8_t* st = stage[w];
   const int t1 = run.t0 + run.n;
-  for (int r = lane; r < 4 * HD; r += 64) {
-    const int g = r / HD;
+  const int sub = tid / LPT, d0 = (tid % LPT) * 8;
+  // K of all passes is on its way while V crosses
+  uint4 kq[PASSES];
+  uint32_t ks[PASSES];
+#pragma unroll
+  for (int q = 0; q < PASSES; ++q) {
+    if (q * TP >= run.n) break;
+    const int t = run.t0 + min(q * TP + sub, run.n - 1);
+    if constexpr (FMT == IFR_KV_FP16) {
+      kq[q] = *reinterpret_cast<const uint4*>(kpart + (size_t)paged_koff(FMT, HD, t, d0) * 2);
+    } else if constexpr (FMT == IFR_KV_INT8) {
+      const uint2 w = *reinterpret_cast<const uint2*>(kpart + paged_koff(FMT, HD, t, d0));
+      kq[q] = make_uint4(w.x, w.y, 0u, 0u);
+      ks[q] = kscale[paged_kscale(FMT, HD, t, 0)];
+    } else {
+      kq[q] = make_uint4(*reinterpret_cast<const uint32_t*>(kpart + paged_koff(FMT, HD, t, d0) / 2), 0u, 0u, 0u);
+      ks[q] = *reinterpret_cast<const uint32_t*>(kscale + paged_kscale(FMT, HD, t, d0 / kPgGroup));
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < VR; ++b) {
+    const int r = tid + 256 * b, g = r / HD;
     const int d = FMT == IFR_KV_FP16 ? r % HD : (r % (HD / 16)) * 16 + (r % HD) / (HD / 16);
     uint32_t x[4];
+    uint4 s = make_uint4(0u, 0u, 0u, 0u), z = s;
     if constexpr (FMT == IFR_KV_FP16) {
       const uint4 q = reinterpret_cast<const uint4*>(vpart)[r];
       x[0] = q.x; x[1] = q.y; x[2] = q.z; x[3] = q.w;
     } else if constexpr (FMT == IFR_KV_INT8) {
       const uint2 q = reinterpret_cast<const uint2*>(vpart)[r];
       x[0] = q.x; x[1] = q.y;
+      s = reinterpret_cast<const uint4*>(vscale)[g];
     } else {
       x[0] = reinterpret_cast<const uint32_t*>(vpart)[r];
+      const uint4* sz = reinterpret_cast<const uint4*>(vscale) + (g * (HD / kPgGroup) + d / kPgGroup) * 2;
+      s = sz[0];
+      z = sz[1];
     }
+    const uint32_t sw[4] = {s.x, s.y, s.z, s.w}, zw[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int t = paged_vtok(g, j);
       if (t < run.t0 || t >= t1) continue;
+      const uint16_t sj = (uint16_t)(sw[j >> 1] >> (16 * (j & 1))), zj = (uint16_t)(zw[j >> 1] >> (16 * (j & 1)));
       uint16_t y;
-      if constexpr (FMT == IFR_KV_FP16) {
-        y = (uint16_t)(x[j >> 1] >> (16 * (j & 1)));
-      } else if constexpr (FMT == IFR_KV_INT8) {
-        y = value_of<FMT>((int)(int8_t)(x[j >> 2] >> (8 * (j & 3))), vscale[paged_vscale(FMT, HD, t, 0)], 0);
-      } else {
-        const int i = paged_vscale(FMT, HD, t, d / kPgGroup);
-        y = value_of<FMT>((int)((x[0] >> (4 * paged_nibble(j))) & 15u), vscale[i], vscale[i + 8]);
-      }
+      if constexpr (FMT == IFR_KV_FP16) y = (uint16_t)(x[j >> 1] >> (16 * (j & 1)));
+      else if constexpr (FMT == IFR_KV_INT8) y = value_of<FMT>((int)(int8_t)(x[j >> 2] >> (8 * (j & 3))), sj, 0);
+      else y = value_of<FMT>((int)((x[0] >> (4 * paged_nibble(j))) & 15u), sj, zj);
       *reinterpret_cast<uint16_t*>(st + t * LROW + d * 2) = y;
     }
   }
-  ifrd::wave_sync();
-  const int sub = lane / LPT, d0 = (lane % LPT) * 8;
-  for (int b = 0; b < run.n; b += TPI) {
-    const int i = b + sub, t = run.t0 + i;
-    if (i >= run.n) continue;
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < PASSES; ++q) {
+    const int i = q * TP + sub, t = run.t0 + i;
+    if (i >= run.n) break;
     const int64_t o = ((int64_t)(run.row + i) * kv.nkv + kvh) * HD + d0;
-    uint4 kw;
-    if constexpr (FMT == IFR_KV_FP16) {
-      kw = *reinterpret_cast<const uint4*>(kpart + (size_t)paged_koff(FMT, HD, t, d0) * 2);
-    } else {
+    uint4 kw = kq[q];
+    if constexpr (FMT != IFR_KV_FP16) {
       uint16_t y[8];
-      if constexpr (FMT == IFR_KV_INT8) {
-        const uint2 c = *reinterpret_cast<const uint2*>(kpart + paged_koff(FMT, HD, t, d0));
-        const uint32_t cw[2] = {c.x, c.y};
-        const uint16_t s = kscale[paged_kscale(FMT, HD, t, 0)];
+      const uint16_t s = (uint16_t)ks[q], z = (uint16_t)(ks[q] >> 16);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = value_of<FMT>((int)(int8_t)(cw[e >> 2] >> (8 * (e & 3))), s, 0);
-      } else {
-        const uint32_t c = *reinterpret_cast<const uint32_t*>(kpart + paged_koff(FMT, HD, t, d0) / 2);
-        const int si = paged_kscale(FMT, HD, t, d0 / kPgGroup);
-        const uint16_t s = kscale[si], z = kscale[si + 1];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = value_of<FMT>((int)((c >> (4 * paged_nibble(e))) & 15u), s, z);
-      }
+      for (int e = 0; e < 8; ++e)
+        y[e] = FMT == IFR_KV_INT8
+                   ? value_of<FMT>((int)(int8_t)((e < 4 ? kw.x : kw.y) >> (8 * (e & 3))), s, 0)
+                   : value_of<FMT>((int)((kw.x >> (4 * paged_nibble(e))) & 15u), s, z);
       kw = make_uint4(y[0] | ((uint32_t)y[1] << 16), y[2] | ((uint32_t)y[3] << 16), y[4] | ((uint32_t)y[5] << 16),
                       y[6] | ((uint32_t)y[7] << 16));
     }
@@ -367,21 +411,21 @@ constexpr int64_t kMaxBlocks = 0x7FFFFFFF;
 
 template <int HD, int FMT>
 hipError_t append_fmt(const PagedAppendArgs& a, const PagedPool& kv, hipStream_t st) {
-  const int64_t kvb = ((int64_t)a.n_runs * kv.nkv + 3) / 4;
-  const int64_t items = a.r.q_d ? (int64_t)a.M * kv.nq * (a.r.rotary / 16 + (HD - a.r.rotary) / 8) : 0;
-  const int64_t blocks = kvb + (items + 255) / 256;
+  const int64_t kvb = (int64_t)a.n_runs * kv.nkv, items = (int64_t)kv.nq * (a.r.rotary / 16 + (HD - a.r.rotary) / 8);
+  const int64_t nr = items < kMaxBlocks ? q_rows((int)items) : 1;
+  const int64_t blocks = kvb + (a.r.q_d ? (a.M + nr - 1) / nr : 0);
   if (blocks <= 0) return hipSuccess;
-  if (blocks > kMaxBlocks) return hipErrorInvalidValue;
+  if (blocks > kMaxBlocks || items > kMaxBlocks) return hipErrorInvalidValue;
   hipLaunchKernelGGL((paged_append_kernel<HD, FMT>), dim3((unsigned)blocks), dim3(256), 0, st, a, kv, (int)kvb);
   return hipGetLastError();
 }
 
 template <int HD, int FMT>
 hipError_t read_fmt(const PagedRun* runs, int n, uint16_t* k, uint16_t* v, const PagedPool& kv, hipStream_t st) {
-  const int64_t blocks = ((int64_t)n * kv.nkv + 3) / 4;
+  const int64_t blocks = (int64_t)n * kv.nkv;
   if (blocks <= 0) return hipSuccess;
   if (blocks > kMaxBlocks) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((paged_read_kernel<HD, FMT>), dim3((unsigned)blocks), dim3(256), 0, st, runs, n, k, v, kv);
+  hipLaunchKernelGGL((paged_read_kernel<HD, FMT>), dim3((unsigned)blocks), dim3(256), 0, st, runs, k, v, kv);
   return hipGetLastError();
 }
 

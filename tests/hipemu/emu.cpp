@@ -393,6 +393,8 @@ int emu_update_dpp(int old, int src, int ctrl, int row_mask, int bank_mask, bool
   } else if (ctrl >= 0x121 && ctrl <= 0x12F) {  // row_ror: lane i reads lane (i - n) mod 16
     const int n = ctrl & 0xF;
     from = (l & ~15) + (((l & 15) - n + 16) & 15);
+  } else if (ctrl == 0x141) {  // row_half_mirror: lane i of 8 reads lane 7 - i
+    from = l ^ 7;
   } else {
     std::fprintf(stderr, "[hipemu] DPP control 0x%x is not emulated\n", ctrl);
     std::abort();

@@ -155,7 +155,7 @@ def refusals(ia, dev):
     plan.set([2, 1], [40, 33], t)
     for over in (dict(k=None), dict(v=None), dict(k=P(a + 2)), dict(v=P(a + 4104)), dict(k_stride=255), dict(k_stride=248),
                  dict(v_stride=260), dict(q=None), dict(q_out=None), dict(q=P(a + 8200)), dict(q_stride=504),
-                 dict(q_out_stride=516), dict(cos=None), dict(sin=None), dict(rotary=8), dict(rotary=144),
+                 dict(q_out_stride=516), dict(cos=None), dict(sin=None), dict(cos=P(a + 32772)), dict(sin=P(a + 40964)), dict(rotary=8), dict(rotary=144),
                  dict(rotary=-16), dict(max_pos=39), dict(q_out=P(a + 8192 + 16)), dict(q_out=P(a)),
                  dict(q_out=P(a + 4096)), dict(k=P(pool.p.value)), dict(v=P(pool.p.value + 4096)),
                  dict(q_out=P(pool.p.value))):
