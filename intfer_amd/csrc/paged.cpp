@@ -38,6 +38,17 @@ constexpr int kWidth[kKinds] = {16, 32, ifrk::kPgWide};
 // each wave of a narrow unit, 256 tokens of a wide one and a step's two pages.
 constexpr int kMinPages[kKinds] = {4, 4, 8}, kGrain[kKinds] = {4, 4, 2};
 constexpr int kCUs = 256;
+// A narrow tile of so few pages is not split: its waves' turns cost less than
+// the launch that joins splits (one row, us: 250 tokens whole 6.2, in two 7.6; 500
+// tokens whole 8.9, in four 8.4).
+constexpr int kWhole = 12;
+// Sequences of more than 32 columns take wide units where the batch has so many
+// pages of wide tiles: below, there are too few of them to hide their longer
+// start, and narrow units, four times as many, win although they turn the pages
+// into fp16 four times (16/8 heads of 128, int4, us narrow / wide: 64 rows on 500
+// tokens 10.9 / 16.0, 256 on 2000, 2112 pages, 23.0 / 27.2, 512 on 2000, 4544,
+// 33.8 / 34.2, 256 on 8000, 8128, 45.8 / 43.1).
+constexpr int64_t kWidePages = 16 * kCUs;
 
 // The context's device is current while a call runs, the caller's afterwards.
 struct OnDevice {
@@ -154,7 +165,7 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
   std::vector<uint8_t> written((size_t)c.n_pages, 0);
   bool appendable = true;
   int max_pos = -1;
-  int64_t m = 0, pages[kKinds] = {};
+  int64_t m = 0;
   for (int s = 0; s < S; ++s) {
     const int n = b->len[s], r = b->rows[s];
     row0[s] = (int)m;
@@ -176,27 +187,43 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
       runs.push_back({pg, t0, k, (int)(m + pos - (n - r)), pos, {0, 0, 0}});
       pos += k;
     }
-    const int64_t ncols = (int64_t)r * G;
-    const int kind = ncols <= 16 ? 0 : ncols <= 32 ? 1 : 2, width = kWidth[kind];
-    for (int64_t c0 = 0; c0 < ncols; c0 += width) {
-      const int nc = (int)std::min<int64_t>(width, ncols - c0);
-      int lo = 0x7FFFFFFF, hi = 0;
-      for (int64_t i = c0 / G; i <= (c0 + nc - 1) / G; ++i) {
-        const ifrk::PagedRow& x = rows[(size_t)(m + i)];
-        if (x.lo >= x.hi) continue;
-        lo = std::min(lo, x.lo);
-        hi = std::max(hi, x.hi);
-      }
-      Tile tl{kind, s, (int)c0, nc, 0, 0};
-      if (lo < hi) {
-        tl.p0 = lo / kPgTok;
-        tl.p1 = (hi + kPgTok - 1) / kPgTok;
-      }
-      pages[kind] += tl.p1 - tl.p0;
-      tiles.push_back(tl);
-    }
     m += r;
   }
+  // The pages that columns [c0, c0 + n) of sequence s look at.
+  const auto tile_of = [&](int kind, int s, int64_t c0, int n) {
+    int lo = 0x7FFFFFFF, hi = 0;
+    for (int64_t i = c0 / G; i <= (c0 + n - 1) / G; ++i) {
+      const ifrk::PagedRow& x = rows[(size_t)(row0[s] + i)];
+      if (x.lo >= x.hi) continue;
+      lo = std::min(lo, x.lo);
+      hi = std::max(hi, x.hi);
+    }
+    Tile t{kind, s, (int)c0, n, 0, 0};
+    if (lo < hi) {
+      t.p0 = lo / kPgTok;
+      t.p1 = (hi + kPgTok - 1) / kPgTok;
+    }
+    return t;
+  };
+  const auto cut = [&](int kind, int s, std::vector<Tile>& to) {
+    const int64_t n = (int64_t)b->rows[s] * G;
+    for (int64_t c0 = 0; c0 < n; c0 += kWidth[kind])
+      to.push_back(tile_of(kind, s, c0, (int)std::min<int64_t>(kWidth[kind], n - c0)));
+  };
+  std::vector<Tile> wide;
+  int64_t wide_pages = 0;
+  for (int s = 0; s < S; ++s)
+    if ((int64_t)b->rows[s] * G > kWidth[1]) cut(2, s, wide);
+  for (const Tile& t : wide) wide_pages += (int64_t)(t.p1 - t.p0) * c.n_kv;
+  const bool use_wide = wide_pages >= kWidePages;
+  if (use_wide) tiles = wide;
+  for (int s = 0; s < S; ++s) {
+    const int64_t n = (int64_t)b->rows[s] * G;
+    if (n == 0 || (n > kWidth[1] && use_wide)) continue;
+    cut(n <= kWidth[0] ? 0 : 1, s, tiles);
+  }
+  int64_t pages[kKinds] = {};
+  for (const Tile& t : tiles) pages[t.kind] += t.p1 - t.p0;
   // Pages of a unit: the fewest for which the batch's units all run at once,
   // so that no CU waits for a last round of few; with more tiles than that, the
   // share of a workgroup.
@@ -228,7 +255,8 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
   std::vector<ifrk::PagedJoin> joins;
   int64_t cols = 0;
   for (const Tile& t : tiles) {
-    const int want = wants[t.kind], np = t.p1 - t.p0, cuts = std::max(1, (np + want - 1) / want);
+    const int want = wants[t.kind], np = t.p1 - t.p0;
+    const int cuts = t.kind < 2 && np <= kWhole ? 1 : std::max(1, (np + want - 1) / want);
     const int g = kGrain[t.kind], step = cuts == 1 ? std::max(np, 1) : ((np + cuts - 1) / cuts + g - 1) / g * g;
     const int ns = std::max(1, (np + step - 1) / step);
     for (int h = 0; h < c.n_kv; ++h) {

@@ -181,10 +181,14 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t x) {  // of two fp16
 }
 
 __device__ __forceinline__ int wave_max_i(int v) {  // uniform, in a scalar register
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v = max(v, __shfl_xor(v, m, 64));
-  return __builtin_amdgcn_readfirstlane(v);
+  v = max(v, ifrd::dpp_i<ifrd::kQuadXor1>(v));
+  v = max(v, ifrd::dpp_i<ifrd::kQuadXor2>(v));
+  v = max(v, ifrd::dpp_i<ifrd::kRowRor4>(v));
+  v = max(v, ifrd::dpp_i<ifrd::kRowRor8>(v));
+  return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
+
 // ---- V of edge pages ----
 // Tokens that no column sees are cleared, and so are values that are not
 // finite: a product with a weight of zero must stay zero.  What a column does
@@ -396,14 +400,12 @@ __global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_na
 #pragma unroll
   for (int t = 0; t < NT; ++t) ub[t].clear();
 
-  struct {
+  struct {  // a lane's part of a page
     uint32_t k[2][I * W];
     uint32_t sz[FMT == IFR_KV_INT4 ? 2 * U : 1];  // int4 [u][h]: scale | minimum; int8: both tiles' scales
-  } kb;
-  struct {
     uint32_t v[N * W];
     uint32_t s[FMT == IFR_KV_INT4 ? U * 8 : 4];   // int4 [u]: 8 scales, 8 minima; int8: 8 scales
-  } vb;
+  } rb;
   const int32_t* tab = a.table + un.tab;
   const size_t page_bytes = paged_page(FMT, HD, kv.nkv), head = (size_t)un.kvh * 2 * kPart;
   // every load is unconditional (the page clamped to the unit's last one)
@@ -413,36 +415,33 @@ __global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_na
     for (int h = 0; h < 2; ++h) {
       if constexpr (FMT == IFR_KV_FP16) {
 #pragma unroll
-        for (int k = 0; k < I; ++k) load_dwords<4>(p + ((4 * k + g) * 32 + 16 * h + c) * 16, &kb.k[h][4 * k]);
+        for (int k = 0; k < I; ++k) load_dwords<4>(p + ((4 * k + g) * 32 + 16 * h + c) * 16, &rb.k[h][4 * k]);
       } else {
-        load_dwords<I * W>(p + ((16 * h + c) * 4 + g) * (I * W * 4), kb.k[h]);
+        load_dwords<I * W>(p + ((16 * h + c) * 4 + g) * (I * W * 4), rb.k[h]);
       }
     }
-    if constexpr (FMT == IFR_KV_INT8) load_dwords<1>(p + kCodes + c * 4, kb.sz);
-    if constexpr (FMT == IFR_KV_INT4) load_dwords<2 * U>(p + kCodes + c * (8 * U), kb.sz);
+    if constexpr (FMT == IFR_KV_INT8) load_dwords<1>(p + kCodes + c * 4, rb.sz);
+    if constexpr (FMT == IFR_KV_INT4) load_dwords<2 * U>(p + kCodes + c * (8 * U), rb.sz);
   };
   auto load_v = [&](const uint8_t* p) {
     p += kPart;
     if constexpr (FMT == IFR_KV_FP16) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) load_dwords<4>(p + (g * HD + 16 * n + c) * 16, &vb.v[4 * n]);
+      for (int n = 0; n < N; ++n) load_dwords<4>(p + (g * HD + 16 * n + c) * 16, &rb.v[4 * n]);
     } else {
-      load_dwords<N * W>(p + (g * 16 + c) * (N * W * 4), vb.v);
-      load_dwords<(FMT == IFR_KV_INT4 ? U * 8 : 4)>(p + kCodes + g * (FMT == IFR_KV_INT4 ? U * 32 : 16), vb.s);
+      load_dwords<N * W>(p + (g * 16 + c) * (N * W * 4), rb.v);
+      load_dwords<(FMT == IFR_KV_INT4 ? U * 8 : 4)>(p + kCodes + g * (FMT == IFR_KV_INT4 ? U * 32 : 16), rb.s);
     }
   };
 
   const int i0 = un.p0 + w;
-  const uint8_t *cur = nullptr, *nxt = nullptr;
   if (i0 < un.p1) {
-    cur = block_of(i0);
-    nxt = block_of(i0 + 4);
-    load_k(cur);
-    load_v(cur);
+    load_k(block_of(i0));
+    load_v(block_of(i0));
   }
 #pragma unroll 1
   for (int i = i0; i < un.p1; i += 4) {
-    const uint8_t* after = block_of(i + 8);  // its table entry is there when it is wanted
+    const uint8_t* const nxt = block_of(i + 4);
     const int t0 = i * kPgTok;
     v4f s[NT][2];
 #pragma unroll
@@ -451,9 +450,9 @@ __global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_na
 #pragma unroll
       for (int k = 0; k < I; ++k) {
         uint32_t sz = 0;
-        if constexpr (FMT == IFR_KV_INT8) sz = h ? kb.sz[0] >> 16 : kb.sz[0];
-        if constexpr (FMT == IFR_KV_INT4) sz = kb.sz[(k / 2) * 2 + h];
-        const v8h kf = k_values<FMT>(&kb.k[h][k * W], sz);
+        if constexpr (FMT == IFR_KV_INT8) sz = h ? rb.sz[0] >> 16 : rb.sz[0];
+        if constexpr (FMT == IFR_KV_INT4) sz = rb.sz[(k / 2) * 2 + h];
+        const v8h kf = k_values<FMT>(&rb.k[h][k * W], sz);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           if (k == 0) s[t][h] = (v4f){0.f, 0.f, 0.f, 0.f};
@@ -516,16 +515,16 @@ __global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_na
       const u4 keep = kept(t0, g, lo_min, hi_max);
       if constexpr (FMT == IFR_KV_FP16) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) edge_run(&vb.v[4 * n], keep, bad);
+        for (int n = 0; n < N; ++n) edge_run(&rb.v[4 * n], keep, bad);
       } else {
 #pragma unroll
-        for (int u = 0; u < (S ? U : 1); ++u) edge_scales<FMT>(&vb.s[u * S], &vb.s[u * S + S / 2], keep, bad);
+        for (int u = 0; u < (S ? U : 1); ++u) edge_scales<FMT>(&rb.s[u * S], &rb.s[u * S + S / 2], keep, bad);
       }
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int u = n / 4;
-      const v8h vf = v_values<FMT>(&vb.v[n * W], &vb.s[u * S], &vb.s[u * S + S / 2]);
+      const v8h vf = v_values<FMT>(&rb.v[n * W], &rb.s[u * S], &rb.s[u * S + S / 2]);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, phi[t], o[t][n], 0, 0, 0);
@@ -542,14 +541,11 @@ __global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_na
           if (!sb) continue;
 #pragma unroll 1
           for (int k = 0; k < 4 * N; ++k)
-            ub[t].template add<HD, FMT>(cur + kPart, e >> 3, e & 7, 16 * (k >> 2) + 4 * g + (k & 3), k);
+            ub[t].template add<HD, FMT>(block_of(i) + kPart, e >> 3, e & 7, 16 * (k >> 2) + 4 * g + (k & 3), k);
         }
       }
     }
-    cur = nxt;
-    nxt = after;
   }
-
 #pragma unroll
   for (int t = 0; t < NT; ++t)
     if (!__all(!ub[t].any()))
