@@ -30,18 +30,20 @@ namespace {
 constexpr int64_t kMaxRows = 1 << 24;      // rows of a batch
 constexpr int64_t kMaxTokens = 1 << 30;    // tokens of a sequence
 
-// Kinds of attention unit: narrow with one and two column tiles, wide.
-constexpr int kKinds = 3;
-constexpr int kWidth[kKinds] = {16, 32, ifrk::kPgWide};
+// Kinds of attention unit, by the columns and the waves of their workgroups:
+// narrow ones of one and two column tiles, wide ones, and narrow ones of two
+// tiles by eight waves.
+constexpr int kKinds = 4, kWide = 2, kEight = 3;
+constexpr int kWidth[kKinds] = {16, 32, ifrk::kPgWide, 32}, kTiles[kKinds] = {1, 2, 0, 2}, kWaves[kKinds] = {4, 4, 4, 8};
 
-// The fewest pages of a split, and what a split is a multiple of: a page for
-// each wave of a narrow unit, 256 tokens of a wide one and a step's two pages.
-constexpr int kMinPages[kKinds] = {4, 4, 8}, kGrain[kKinds] = {4, 4, 2};
+// The fewest pages of a wide split (256 tokens) and what one is a multiple of (a
+// step's two pages); narrow: a page for each wave.
+constexpr int kWideMin = 8, kWideGrain = 2;
 constexpr int kCUs = 256;
-// A narrow tile of so few pages is not split: its waves' turns cost less than
-// the launch that joins splits (one row, us: 250 tokens whole 6.2, in two 7.6; 500
-// tokens whole 8.9, in four 8.4).
-constexpr int kWhole = 12;
+// A narrow tile of so few pages a wave is not split: its waves' turns cost less
+// than the launch that joins splits (one row, four waves, us: 250 tokens whole
+// 5.6, in two 7.6; 500 tokens whole 8.9, in four 8.4).
+constexpr int kWhole = 3;
 // Sequences of more than 32 columns take wide units where the batch has so many
 // pages of wide tiles: below, there are too few of them to hide their longer
 // start, and narrow units, four times as many, win although they turn the pages
@@ -49,6 +51,13 @@ constexpr int kWhole = 12;
 // tokens 10.9 / 16.0, 256 on 2000, 2112 pages, 23.0 / 27.2, 512 on 2000, 4544,
 // 33.8 / 34.2, 256 on 8000, 8128, 45.8 / 43.1).
 constexpr int64_t kWidePages = 16 * kCUs;
+// Two-tile units of heads of 128 leave a CU eight waves.  One workgroup of all
+// of them takes whole tiles where two of four would need splits and a join: if
+// the CUs hold all tiles at once and the longest is not far over the mean, or is
+// whole for eight waves and not for four (16/8 heads of 128, int4: 512 rows on 500
+// tokens 20.9 -> 15.9 us, 128 on 500 13.9 -> 11.2; but 28 x 5 verify rows on ragged
+// contexts, the longest twice the mean, 28.0 -> 34.7).
+constexpr double kEven = 1.5;
 
 // The context's device is current while a call runs, the caller's afterwards.
 struct OnDevice {
@@ -213,7 +222,7 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
   std::vector<Tile> wide;
   int64_t wide_pages = 0;
   for (int s = 0; s < S; ++s)
-    if ((int64_t)b->rows[s] * G > kWidth[1]) cut(2, s, wide);
+    if ((int64_t)b->rows[s] * G > kWidth[1]) cut(kWide, s, wide);
   for (const Tile& t : wide) wide_pages += (int64_t)(t.p1 - t.p0) * c.n_kv;
   const bool use_wide = wide_pages >= kWidePages;
   if (use_wide) tiles = wide;
@@ -222,32 +231,41 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
     if (n == 0 || (n > kWidth[1] && use_wide)) continue;
     cut(n <= kWidth[0] ? 0 : 1, s, tiles);
   }
-  int64_t pages[kKinds] = {};
-  for (const Tile& t : tiles) pages[t.kind] += t.p1 - t.p0;
+  int64_t pages[kKinds] = {}, n_tiles[kKinds] = {}, most[kKinds] = {};
+  for (const Tile& t : tiles) {
+    pages[t.kind] += t.p1 - t.p0;
+    most[t.kind] = std::max<int64_t>(most[t.kind], t.p1 - t.p0);
+    ++n_tiles[t.kind];
+  }
+  const int64_t eight = kCUs * ifrk::paged_narrow_waves(c.format, c.head_dim, 2) / 2;  // workgroups at once
+  if (c.head_dim == 128 && n_tiles[1] * c.n_kv <= eight &&
+      ((double)most[1] * eight <= kEven * (double)pages[1] * c.n_kv ||
+       (most[1] > 4 * kWhole && most[1] <= 8 * kWhole))) {
+    for (Tile& t : tiles)
+      if (t.kind == 1) t.kind = kEight;
+    std::swap(pages[1], pages[kEight]);
+    std::swap(most[1], most[kEight]);
+    std::swap(n_tiles[1], n_tiles[kEight]);
+  }
   // Pages of a unit: the fewest for which the batch's units all run at once,
   // so that no CU waits for a last round of few; with more tiles than that, the
   // share of a workgroup.
-  int wants[kKinds];
+  int wants[kKinds], grains[kKinds];
   for (int k = 0; k < kKinds; ++k) {
-    const int64_t slots = kCUs * (k < 2 ? ifrk::paged_narrow_waves(c.format, c.head_dim, k + 1)
-                                        : ifrk::paged_wide_groups(c.head_dim));
-    const auto grain = [&](int64_t n) { return (int)std::max<int64_t>(kMinPages[k], (n + kGrain[k] - 1) / kGrain[k] * kGrain[k]); };
-    int64_t most = 0, n_tiles = 0;
-    for (const Tile& t : tiles)
-      if (t.kind == k) {
-        most = std::max<int64_t>(most, t.p1 - t.p0);
-        ++n_tiles;
-      }
+    const int64_t slots = k == kWide ? kCUs * ifrk::paged_wide_groups(c.head_dim)
+                                     : kCUs * ifrk::paged_narrow_waves(c.format, c.head_dim, kTiles[k]) * 4 / kWaves[k];
+    const int g = grains[k] = k == kWide ? kWideGrain : kWaves[k], least = k == kWide ? kWideMin : kWaves[k];
+    const auto grain = [&](int64_t n) { return (int)std::max<int64_t>(least, (n + g - 1) / g * g); };
     const int64_t share = (pages[k] * c.n_kv + slots - 1) / slots;
-    int lo = grain(share), hi = std::max(lo, grain(most));
-    if (n_tiles * c.n_kv <= slots)
+    int lo = grain(share), hi = std::max(lo, grain(most[k]));
+    if (n_tiles[k] * c.n_kv <= slots)
       while (lo < hi) {
-        const int mid = lo + (hi - lo) / kGrain[k] / 2 * kGrain[k];
+        const int mid = lo + (hi - lo) / g / 2 * g;
         int64_t units = 0;
         for (const Tile& t : tiles)
           if (t.kind == k) units += std::max(1, (t.p1 - t.p0 + mid - 1) / mid);
         if (units * c.n_kv <= slots) hi = mid;
-        else lo = mid + kGrain[k];
+        else lo = mid + g;
       }
     wants[k] = lo;
   }
@@ -256,8 +274,8 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
   int64_t cols = 0;
   for (const Tile& t : tiles) {
     const int want = wants[t.kind], np = t.p1 - t.p0;
-    const int cuts = t.kind < 2 && np <= kWhole ? 1 : std::max(1, (np + want - 1) / want);
-    const int g = kGrain[t.kind], step = cuts == 1 ? std::max(np, 1) : ((np + cuts - 1) / cuts + g - 1) / g * g;
+    const int cuts = t.kind != kWide && np <= kWhole * grains[t.kind] ? 1 : std::max(1, (np + want - 1) / want);
+    const int g = grains[t.kind], step = cuts == 1 ? std::max(np, 1) : ((np + cuts - 1) / cuts + g - 1) / g * g;
     const int ns = std::max(1, (np + step - 1) / step);
     for (int h = 0; h < c.n_kv; ++h) {
       const int64_t base = cols;
@@ -510,7 +528,8 @@ int ifr_paged_attention(ifr_paged* p, const void* pool_d, const ifr_paged_query*
   for (int k = 0; k < kKinds; ++k) {
     a.units = reinterpret_cast<const ifrk::PagedUnit*>(p->meta + p->o_units[k]);
     a.n_units = p->n_units[k];
-    PGCHK(k < 2 ? ifrk::launch_paged_narrow(a, kv, k + 1, p->st) : ifrk::launch_paged_wide(a, kv, p->st));
+    PGCHK(k == kWide ? ifrk::launch_paged_wide(a, kv, p->st)
+                     : ifrk::launch_paged_narrow(a, kv, kTiles[k], kWaves[k], p->st));
   }
   PGCHK(ifrk::launch_paged_join(reinterpret_cast<const ifrk::PagedJoin*>(p->meta + p->o_joins), p->n_joins, a, kv,
                                 p->st));

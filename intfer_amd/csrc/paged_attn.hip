@@ -116,53 +116,62 @@ __device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t* w) {
 
 // What a score becomes: in x[C] q.k, out the score times log2 e.
 //
-// cap tanh(a / cap) keeps errors relative to the result, so that small scores
-// keep their bits.  While every |a / cap| of the wave is at most 1/2 (scores
-// hardly ever come near their cap) it is x P(x^2), P the degree-4 Chebyshev
-// interpolation of tanh(x) / x in x^2 on [0, 1/4] (1.4e-8 off), 7 operations a
-// score with the factors inside; else 1 - 2 / (e^2x + 1) above 1/2.  The bias takes |pos - t| in fp32,
-// exact up to 2^24; far(j) is pos - t of score j.
+// cap tanh(z), z = scale q.k / cap, keeps errors relative to the result, so that
+// small scores keep their bits.  While every |z| of the wave is at most 1/2
+// (scores hardly ever come near their cap) it is z P(z^2), P the Chebyshev
+// interpolation of tanh(z) / z in z^2 on [0, 1/4]: of degree 4 (1.4e-8 off) for
+// fp32 outputs, 3 (6e-7, where the rounding of P and of the output is 2e-4) for
+// fp16 ones, with every factor inside the coefficients: 5 or 6 operations a
+// score.  Else, and where a power of scale / cap would leave fp32, 1 - 2 / (e^2z
+// + 1) above 1/2.  The bias takes |pos - t| in fp32, exact up to 2^24; far(j) is
+// pos - t of score j.
 struct Scoring {
   float scale2;           // scale log2 e
   float inv, cap2;        // scale / cap, cap log2 e; inv 0: no cap
-  float c[5];             // cap2 P
+  float limit;            // |q.k| up to which f holds (negative: none)
+  float f[5];             // cap2 P, times the powers of inv
   bool mod;               // cap or bias
 };
+constexpr float kTanh4[5] = {0.99999999f, -0.333330679f, 0.133247505f, -0.0529842388f, 0.0171313444f};
+constexpr float kTanh3[5] = {0.999999451f, -0.333262842f, 0.131899394f, -0.0443927384f, 0.0f};
+template <bool FINE>
 __device__ __forceinline__ Scoring scoring(const PagedAttnArgs& a) {
   Scoring s;
   s.scale2 = a.scale * kLog2e;
   s.inv = a.cap != 0.0f ? a.scale / a.cap : 0.0f;
   s.cap2 = a.cap * kLog2e;
-  s.c[0] = 0.99999999f * s.cap2;
-  s.c[1] = -0.333330679f * s.cap2;
-  s.c[2] = 0.133247505f * s.cap2;
-  s.c[3] = -0.0529842388f * s.cap2;
-  s.c[4] = 0.0171313444f * s.cap2;
+  s.limit = s.inv >= 1e-4f && s.inv <= 1e3f ? 0.5f / s.inv : -1.0f;
+  float w = s.cap2 * s.inv;
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    s.f[i] = (FINE ? kTanh4[i] : kTanh3[i]) * w;
+    w *= s.inv * s.inv;
+  }
   s.mod = a.cap != 0.0f || a.slopes != nullptr;
   return s;
 }
-template <int C, typename Far>
+template <bool FINE, int C, typename Far>
 __device__ __forceinline__ void modify(float (&x)[C], const Scoring& s, bool biased, float slope2, Far far) {
   if (s.inv != 0.0f) {
     float big = 0.0f;
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      x[j] *= s.inv;
-      big = fmaxf(big, fabsf(x[j]));
-    }
-    auto poly = [&](float v) {
-      const float y = v * v;
-      return v * fmaf(fmaf(fmaf(fmaf(s.c[4], y, s.c[3]), y, s.c[2]), y, s.c[1]), y, s.c[0]);
-    };
-    if (__all(!(big > 0.5f))) {
+    for (int j = 0; j < C; ++j) big = fmaxf(big, fabsf(x[j]));
+    if (__all(!(big > s.limit))) {
 #pragma unroll
-      for (int j = 0; j < C; ++j) x[j] = poly(x[j]);
+      for (int j = 0; j < C; ++j) {
+        const float y = x[j] * x[j];
+        float p = fmaf(s.f[3], y, s.f[2]);
+        if constexpr (FINE) p = fmaf(fmaf(s.f[4], y, s.f[3]), y, s.f[2]);
+        x[j] *= fmaf(fmaf(p, y, s.f[1]), y, s.f[0]);
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        const float e = __builtin_amdgcn_exp2f(fabsf(x[j]) * (2.0f * kLog2e));
-        const float t = __builtin_copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f), x[j]);
-        x[j] = fabsf(x[j]) > 0.5f ? t * s.cap2 : poly(x[j]);
+        const float z = x[j] * s.inv, y = z * z;
+        const float e = __builtin_amdgcn_exp2f(fabsf(z) * (2.0f * kLog2e));
+        const float t = __builtin_copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f), z);
+        const float p = fmaf(fmaf(fmaf(fmaf(kTanh4[4], y, kTanh4[3]), y, kTanh4[2]), y, kTanh4[1]), y, kTanh4[0]);
+        x[j] = (fabsf(z) > 0.5f ? t : z * p) * s.cap2;
         __builtin_amdgcn_sched_barrier(0);  // (one at a time: the seldom case is to hold few registers)
       }
     }
@@ -329,7 +338,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedJoin* joins,
                    ifrd::f2h(x[2]) | ((uint32_t)ifrd::f2h(x[3]) << 16));
 }
 
-// ---- few columns: the four waves of a workgroup take every fourth page ------------------------
+// ---- few columns: the waves of a workgroup take the pages in turn --------------------------------
 //
 // A wave holds NT tiles of 16 columns.  The next page's K is loaded once the
 // first product has read this one's, its V once the second product has.  At
@@ -341,8 +350,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedJoin* joins,
 // 57.3 us, 16 of 32000 160.6 -> 152.3).  Bound by its VALU work at 4 bits:
 // 13 operations turn a dword of codes into 8 values.  (Two K buffers and both
 // steps unrolled spilled at 192 VGPRs: 142.8 and 467 us.)
-template <int HD, int FMT, int NT, bool HL>
-__global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_narrow_kernel(PagedAttnArgs a, PagedPool kv) {
+template <int HD, int FMT, int NT, int NW, bool HL>
+__global__ __launch_bounds__(64 * NW, paged_narrow_waves(FMT, HD, NT)) void paged_narrow_kernel(PagedAttnArgs a, PagedPool kv) {
   constexpr int I = HD / 32, N = HD / 16, U = HD / kPgGroup;
   constexpr int W = FMT == IFR_KV_FP16 ? 4 : FMT == IFR_KV_INT8 ? 2 : 1;  // dwords of 8 elements
   constexpr size_t kPart = paged_part(FMT, HD);
@@ -351,7 +360,7 @@ __global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_na
   const int c = lane & 15, g = lane >> 4;
   const PagedUnit un = a.units[blockIdx.x];
   const int G = kv.nq / kv.nkv;
-  const Scoring sco = scoring(a);
+  const Scoring sco = scoring<HL>(a);
   const float sl = sco.mod ? 1.0f : sco.scale2;  // what turns a score into powers of two
 
   v8h qf[NT][I];
@@ -440,8 +449,8 @@ __global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_na
     load_v(block_of(i0));
   }
 #pragma unroll 1
-  for (int i = i0; i < un.p1; i += 4) {
-    const uint8_t* const nxt = block_of(i + 4);
+  for (int i = i0; i < un.p1; i += NW) {
+    const uint8_t* const nxt = block_of(i + NW);
     const int t0 = i * kPgTok;
     v4f s[NT][2];
 #pragma unroll
@@ -471,7 +480,7 @@ __global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_na
       for (int j = 0; j < 8; ++j) x[j] = s[t][j >> 2][j & 3];
       if (sco.mod) {
         const float d = (float)(pos[t] - t0 - 4 * g);
-        modify(x, sco, a.slopes != nullptr, slope[t], [&](int j) { return d - (float)(16 * (j >> 2) + (j & 3)); });
+        modify<HL>(x, sco, a.slopes != nullptr, slope[t], [&](int j) { return d - (float)(16 * (j >> 2) + (j & 3)); });
       }
       seen[t] = 0xFFu;
       if (!inner) {
@@ -552,11 +561,11 @@ __global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_na
 #pragma unroll
       for (int k = 0; k < 4 * N; ++k) o[t][k >> 2][k & 3] = ub[t].value(k, o[t][k >> 2][k & 3]);
 
-  // ---- the four waves' parts: the columns' common maximum first, then O in
+  // ---- the waves' parts: the columns' common maximum first, then O in
   // slices of 64 dims
   constexpr int kRow = 68;  // floats of a column in a slice (16 lanes' stores on 64 banks)
-  __shared__ __align__(16) float slab[4][16 * NT * kRow];
-  __shared__ float ml[4][16 * NT][2];
+  __shared__ __align__(16) float slab[NW][16 * NT * kRow];
+  __shared__ float ml[NW][16 * NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     l_run[t] += ifrd::lane_xor<16>(l_run[t]);
@@ -572,10 +581,10 @@ __global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_na
   for (int t = 0; t < NT; ++t) {
     float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) m = fmaxf(m, ml[q][16 * t + c][0]);
+    for (int q = 0; q < NW; ++q) m = fmaxf(m, ml[q][16 * t + c][0]);
     const float mu = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) l += __builtin_amdgcn_exp2f(ml[q][16 * t + c][0] - mu) * ml[q][16 * t + c][1];
+    for (int q = 0; q < NW; ++q) l += __builtin_amdgcn_exp2f(ml[q][16 * t + c][0] - mu) * ml[q][16 * t + c][1];
     f[t] = __builtin_amdgcn_exp2f(m_run[t] - mu);
     if (un.part < 0) {
       f[t] = l == 0.0f ? 0.0f : f[t] / l;  // a row that sees nothing: zeros
@@ -595,13 +604,14 @@ __global__ __launch_bounds__(256, paged_narrow_waves(FMT, HD, NT)) void paged_na
       for (int n = 0; n < 4; ++n)
         *reinterpret_cast<v4f*>(&slab[w][(16 * t + c) * kRow + 16 * n + 4 * g]) = o[t][4 * q + n] * f[t];
     __syncthreads();
+    // 16 lanes a column, 4 dims each; NW x 4 columns at once
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int i = 16 * t + tid / 16, d = (tid % 16) * 4;
+    for (int t = 0; t < (4 * NT + NW - 1) / NW; ++t) {
+      const int i = 4 * NW * t + tid / 16, d = (tid % 16) * 4;
       if (i >= un.ncol) continue;
       v4f x = *reinterpret_cast<const v4f*>(&slab[0][i * kRow + d]);
 #pragma unroll
-      for (int k = 1; k < 4; ++k) x += *reinterpret_cast<const v4f*>(&slab[k][i * kRow + d]);
+      for (int k = 1; k < NW; ++k) x += *reinterpret_cast<const v4f*>(&slab[k][i * kRow + d]);
       if (un.part >= 0) {
         *reinterpret_cast<v4f*>(a.part_o + ((int64_t)un.part + i) * HD + 64 * q + d) = x;
       } else {
@@ -652,7 +662,7 @@ __global__ __launch_bounds__(256, paged_wide_groups(HD)) void paged_wide_kernel(
   const int c = lane & 31, hl = lane >> 5;
   const PagedUnit un = a.units[blockIdx.x];
   const int G = kv.nq / kv.nkv;
-  const Scoring sco = scoring(a);
+  const Scoring sco = scoring<HL>(a);
   const float sl = sco.mod ? 1.0f : sco.scale2;
 
   // this lane's column
@@ -799,7 +809,7 @@ __global__ __launch_bounds__(256, paged_wide_groups(HD)) void paged_wide_kernel(
     for (int r = 0; r < 16; ++r) x[r] = s[r];
     if (sco.mod) {
       const float d = (float)(pos - t0 - 4 * hl);
-      modify(x, sco, a.slopes != nullptr, slope, [&](int r) { return d - (float)wide_tok(8 * (r >> 2) + (r & 3)); });
+      modify<HL>(x, sco, a.slopes != nullptr, slope, [&](int r) { return d - (float)wide_tok(8 * (r >> 2) + (r & 3)); });
     }
     uint32_t seen = 0xFFFFu;
     if (!inner) {
@@ -901,15 +911,21 @@ __global__ __launch_bounds__(256, paged_wide_groups(HD)) void paged_wide_kernel(
     }
 }
 
-template <int HD, int FMT>
-hipError_t narrow_fmt(const PagedAttnArgs& a, const PagedPool& kv, int tiles, hipStream_t st) {
-  const dim3 grid(a.n_units), block(256);
-  if (tiles == 1 && a.out_f32) hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, 1, true>), grid, block, 0, st, a, kv);
-  else if (tiles == 1) hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, 1, false>), grid, block, 0, st, a, kv);
-  else if (tiles == 2 && a.out_f32) hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, 2, true>), grid, block, 0, st, a, kv);
-  else if (tiles == 2) hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, 2, false>), grid, block, 0, st, a, kv);
-  else return hipErrorInvalidValue;
+template <int HD, int FMT, int NT, int NW>
+hipError_t narrow_shape(const PagedAttnArgs& a, const PagedPool& kv, hipStream_t st) {
+  const dim3 grid(a.n_units), block(64 * NW);
+  if (a.out_f32) hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, NT, NW, true>), grid, block, 0, st, a, kv);
+  else hipLaunchKernelGGL((paged_narrow_kernel<HD, FMT, NT, NW, false>), grid, block, 0, st, a, kv);
   return hipGetLastError();
+}
+
+template <int HD, int FMT>
+hipError_t narrow_fmt(const PagedAttnArgs& a, const PagedPool& kv, int tiles, int waves, hipStream_t st) {
+  if (tiles == 1 && waves == 4) return narrow_shape<HD, FMT, 1, 4>(a, kv, st);
+  if (tiles == 2 && waves == 4) return narrow_shape<HD, FMT, 2, 4>(a, kv, st);
+  if constexpr (HD == 128)
+    if (tiles == 2 && waves == 8) return narrow_shape<HD, FMT, 2, 8>(a, kv, st);
+  return hipErrorInvalidValue;
 }
 
 template <int HD, int FMT>
@@ -933,33 +949,33 @@ hipError_t wide_fmt(const PagedAttnArgs& a, const PagedPool& kv, hipStream_t st)
 #if defined(IFR_PAGED_FMT)
 // compiled once per format: that format's kernels
 template <int FMT>
-hipError_t paged_narrow_of(const PagedAttnArgs& a, const PagedPool& kv, int tiles, hipStream_t st) {
-  IFR_PAGED_DIMS(narrow_fmt, FMT, a, kv, tiles, st);
+hipError_t paged_narrow_of(const PagedAttnArgs& a, const PagedPool& kv, int tiles, int waves, hipStream_t st) {
+  IFR_PAGED_DIMS(narrow_fmt, FMT, a, kv, tiles, waves, st);
 }
 template <int FMT>
 hipError_t paged_wide_of(const PagedAttnArgs& a, const PagedPool& kv, hipStream_t st) {
   IFR_PAGED_DIMS(wide_fmt, FMT, a, kv, st);
 }
-template hipError_t paged_narrow_of<IFR_PAGED_FMT>(const PagedAttnArgs&, const PagedPool&, int, hipStream_t);
+template hipError_t paged_narrow_of<IFR_PAGED_FMT>(const PagedAttnArgs&, const PagedPool&, int, int, hipStream_t);
 template hipError_t paged_wide_of<IFR_PAGED_FMT>(const PagedAttnArgs&, const PagedPool&, hipStream_t);
 #else
 // and once without: the joins and the dispatch
 template <int FMT>
-hipError_t paged_narrow_of(const PagedAttnArgs& a, const PagedPool& kv, int tiles, hipStream_t st);
+hipError_t paged_narrow_of(const PagedAttnArgs& a, const PagedPool& kv, int tiles, int waves, hipStream_t st);
 template <int FMT>
 hipError_t paged_wide_of(const PagedAttnArgs& a, const PagedPool& kv, hipStream_t st);
 #define IFR_PAGED_EXTERN(FMT)                                                                              \
-  extern template hipError_t paged_narrow_of<FMT>(const PagedAttnArgs&, const PagedPool&, int, hipStream_t); \
+  extern template hipError_t paged_narrow_of<FMT>(const PagedAttnArgs&, const PagedPool&, int, int, hipStream_t); \
   extern template hipError_t paged_wide_of<FMT>(const PagedAttnArgs&, const PagedPool&, hipStream_t)
 IFR_PAGED_EXTERN(IFR_KV_FP16);
 IFR_PAGED_EXTERN(IFR_KV_INT8);
 IFR_PAGED_EXTERN(IFR_KV_INT4);
 
-hipError_t launch_paged_narrow(const PagedAttnArgs& a, const PagedPool& kv, int tiles, hipStream_t st) {
+hipError_t launch_paged_narrow(const PagedAttnArgs& a, const PagedPool& kv, int tiles, int waves, hipStream_t st) {
   if (a.n_units <= 0) return hipSuccess;
-  if (kv.fmt == IFR_KV_FP16) return paged_narrow_of<IFR_KV_FP16>(a, kv, tiles, st);
-  if (kv.fmt == IFR_KV_INT8) return paged_narrow_of<IFR_KV_INT8>(a, kv, tiles, st);
-  if (kv.fmt == IFR_KV_INT4) return paged_narrow_of<IFR_KV_INT4>(a, kv, tiles, st);
+  if (kv.fmt == IFR_KV_FP16) return paged_narrow_of<IFR_KV_FP16>(a, kv, tiles, waves, st);
+  if (kv.fmt == IFR_KV_INT8) return paged_narrow_of<IFR_KV_INT8>(a, kv, tiles, waves, st);
+  if (kv.fmt == IFR_KV_INT4) return paged_narrow_of<IFR_KV_INT4>(a, kv, tiles, waves, st);
   return hipErrorInvalidValue;
 }
 
