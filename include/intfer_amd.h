@@ -296,9 +296,11 @@ int ifr_quant_gemm_ga(ifr_ctx* ctx, const ifr_dlinear* w, const int8_t* a_d, con
  * They run on the context's stream in call order and allocate nothing, so
  * they can be captured into a graph; ifr_paged_set cannot (IFR_ESTATE), and
  * a plan whose calls were captured refuses another ifr_paged_set, because
- * the graph keeps that batch's launches.  Replays of graphs captured from
- * one plan share its workspace: keep them on one stream.  The context's
- * device is made current for the call and the caller's restored.
+ * the graph keeps that batch's launches.  Such a plan outlives its graphs, and
+ * replays of graphs captured from one plan share its workspace: keep them on
+ * one stream.  The context's device is made current for the call and the
+ * caller's restored.  Work on other streams is ordered by the caller, through
+ * ifr_ctx_stream.
  * ---------------------------------------------------------------------- */
 enum {
   IFR_KV_FP16 = 0, /* fp16 */
@@ -346,9 +348,10 @@ int ifr_paged_destroy(ifr_paged* p);
  * rows[s] new rows (0: it takes no part), which are its last positions, len[s]
  * - rows[s] .. len[s] - 1; the batch's rows are those of sequence 0, then of
  * sequence 1, and so on.  Entry i of a sequence's table row is the page of
- * positions 32 i .. 32 i + 31; pages may be shared for reading, but a page
- * that two sequences of the batch (or two entries of one) would write makes
- * ifr_paged_append return IFR_EINVAL.
+ * positions 32 i .. 32 i + 31 (the entries up to len are checked against
+ * n_pages); pages may be shared for reading, but a page that two sequences of
+ * the batch (or two entries of one) would write makes ifr_paged_append return
+ * IFR_EINVAL.
  * A row at position pos sees the positions t with
  *   first <= t < max(pos + 1, prefix),  t < len
  * first: per row, the start of its document or window (NULL: 0); prefix: per

@@ -29,6 +29,7 @@ namespace {
 
 constexpr int64_t kMaxRows = 1 << 24;      // rows of a batch
 constexpr int64_t kMaxTokens = 1 << 30;    // tokens of a sequence
+constexpr int64_t kMaxUnits = 1 << 24;     // attention tiles of all kv heads
 
 // Kinds of attention unit, by the columns and the waves of their workgroups:
 // narrow ones of one and two column tiles, wide ones, and narrow ones of two
@@ -153,6 +154,7 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
   if (S && (!b->rows || !b->len || !b->table)) return fail(IFR_EINVAL, "paged batch: rows, len or table is null");
   int64_t M = 0;
   for (int s = 0; s < S; ++s) {
+    if (b->rows[s] == 0) continue;
     if (b->rows[s] < 0 || b->len[s] < b->rows[s] || b->len[s] > kMaxTokens)
       return fail(IFR_EINVAL, "sequence %d: %d new rows of %d tokens", s, b->rows[s], b->len[s]);
     const int np = (b->len[s] + kPgTok - 1) / kPgTok;
@@ -171,8 +173,7 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
   std::vector<int32_t> table;
   std::vector<Tile> tiles;
   std::vector<int> row0(S), tab(S);
-  std::vector<uint8_t> written((size_t)c.n_pages, 0);
-  bool appendable = true;
+  std::vector<int> written;
   int max_pos = -1;
   int64_t m = 0;
   for (int s = 0; s < S; ++s) {
@@ -191,13 +192,14 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
     max_pos = std::max(max_pos, n - 1);
     for (int pos = n - r; pos < n;) {
       const int t0 = pos % kPgTok, k = std::min(kPgTok - t0, n - pos), pg = t[pos / kPgTok];
-      if (written[pg]) appendable = false;
-      written[pg] = 1;
+      written.push_back(pg);
       runs.push_back({pg, t0, k, (int)(m + pos - (n - r)), pos, {0, 0, 0}});
       pos += k;
     }
     m += r;
   }
+  std::sort(written.begin(), written.end());
+  const bool appendable = std::adjacent_find(written.begin(), written.end()) == written.end();
   // The pages that columns [c0, c0 + n) of sequence s look at.
   const auto tile_of = [&](int kind, int s, int64_t c0, int n) {
     int lo = 0x7FFFFFFF, hi = 0;
@@ -231,6 +233,8 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
     if (n == 0 || (n > kWidth[1] && use_wide)) continue;
     cut(n <= kWidth[0] ? 0 : 1, s, tiles);
   }
+  if ((int64_t)tiles.size() * c.n_kv > kMaxUnits || (int64_t)runs.size() * c.n_kv > kMaxTokens)
+    return fail(IFR_EINVAL, "%lld rows of %d kv heads are too many for one batch", (long long)M, c.n_kv);
   int64_t pages[kKinds] = {}, n_tiles[kKinds] = {}, most[kKinds] = {};
   for (const Tile& t : tiles) {
     pages[t.kind] += t.p1 - t.p0;
@@ -499,7 +503,9 @@ int ifr_paged_attention(ifr_paged* p, const void* pool_d, const ifr_paged_query*
   if (!q) return fail(IFR_EINVAL, "query is null");
   const ifr_paged_cfg& c = p->cfg;
   if (!(q->scale >= 0.0f) || !std::isfinite(q->scale)) return fail(IFR_EINVAL, "scale %g", q->scale);
-  if (!(q->softcap >= 0.0f) || !std::isfinite(q->softcap)) return fail(IFR_EINVAL, "softcap %g", q->softcap);
+  const float scale = q->scale > 0.0f ? q->scale : 1.0f / std::sqrt((float)c.head_dim);
+  if (!(q->softcap >= 0.0f) || !std::isfinite(q->softcap) || (q->softcap > 0.0f && !std::isfinite(scale / q->softcap)))
+    return fail(IFR_EINVAL, "softcap %g", q->softcap);
   if (q->out_f32 != 0 && q->out_f32 != 1) return fail(IFR_EINVAL, "out_f32 %d", q->out_f32);
   if (p->M == 0) return IFR_OK;
   const int64_t w = (int64_t)c.n_heads * c.head_dim, pb = (int64_t)pool_bytes(c);
@@ -519,7 +525,7 @@ int ifr_paged_attention(ifr_paged* p, const void* pool_d, const ifr_paged_query*
   a.out = q->out_d;
   a.out_stride = q->out_stride;
   a.out_f32 = q->out_f32;
-  a.scale = q->scale > 0.0f ? q->scale : 1.0f / std::sqrt((float)c.head_dim);
+  a.scale = scale;
   a.cap = q->softcap;
   a.slopes = q->slopes_d;
   a.part_o = p->part;

@@ -144,6 +144,8 @@ def refusals(ia, dev):
     assert bad_set([41, 1], [40, 33], t) == I         # more new rows than tokens
     assert bad_set([1, 1], [40, 33], t, prefix=[0, -1]) == I
     assert L.ifr_paged_set(plan.h, None) == I and L.ifr_paged_set(None, C.byref(_abi.PagedBatch())) == I
+    # a sequence without new rows takes no part, whatever stands in its entries
+    assert bad_set([1, 0], [40, -3], np.array([[0, 1], [99, -7]])) == ia.IFR_OK
     assert bad_set([], [], np.zeros((0, 0))) == ia.IFR_OK  # an empty batch: calls do nothing
     assert L.ifr_paged_append(plan.h, pool.p, rows()) == ia.IFR_OK
     assert L.ifr_paged_attention(plan.h, pool.p, query()) == ia.IFR_OK
@@ -163,6 +165,7 @@ def refusals(ia, dev):
     for over in (dict(q=None), dict(out=None), dict(q=P(a + 8)), dict(out=P(a + 32776)), dict(q_stride=511),
                  dict(q_stride=504), dict(out_stride=508), dict(out_f32=2), dict(scale=-1.0), dict(scale=float("nan")),
                  dict(scale=float("inf")), dict(softcap=-1.0), dict(softcap=float("inf")), dict(softcap=float("nan")),
+                 dict(softcap=1e-44),
                  dict(out=P(a)), dict(out=P(a + 1024)), dict(out=P(pool.p.value + 64))):
         assert L.ifr_paged_attention(plan.h, pool.p, query(**over)) == I, over
     for k, v in ((None, P(a)), (P(a), None), (P(a + 2), P(a + 4096)), (P(a), P(a + 256)), (P(a), P(pool.p.value))):

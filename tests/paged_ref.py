@@ -1,5 +1,6 @@
 """The caller-owned paged KV cache in numpy, from the formulas of
 include/intfer_amd.h, in float64: what the paged tests hold the kernels to."""
+import functools
 import math
 
 import numpy as np
@@ -18,6 +19,7 @@ def _td(hd):
     return np.arange(PAGE)[:, None], np.arange(hd)[None, :]
 
 
+@functools.lru_cache(None)
 def element(fmt, hd, v):
     """Element number of (token, dim) in a K or V part."""
     t, d = _td(hd)
@@ -31,6 +33,7 @@ def element(fmt, hd, v):
     return ((g * 16 + d % 16) * (hd // 16) + d // 16) * 8 + j
 
 
+@functools.lru_cache(None)
 def scale_index(fmt, hd, v):
     """fp16 index of the scale of (token, dim) behind the codes; the minimum's offset."""
     t, d = _td(hd)
@@ -112,9 +115,9 @@ def write_token(part, fmt, hd, v, t, x):
         return
     sc[i[t] + off] = z[0]
     nib = e // 8 * 8 + 4 * (e % 2) + e % 8 // 2
-    for n, k in zip(nib, c[0]):
-        b = int(part[n // 2])
-        part[n // 2] = (b & 0x0F) | (int(k) << 4) if n % 2 else (b & 0xF0) | int(k)
+    lo, hi = nib % 2 == 0, nib % 2 == 1
+    part[nib[lo] // 2] = (part[nib[lo] // 2] & 0xF0) | c[0, lo]
+    part[nib[hi] // 2] = (part[nib[hi] // 2] & 0x0F) | (c[0, hi] << 4)
 
 
 def tables(max_pos, rotary, theta=1e6):
@@ -189,30 +192,34 @@ def attention(q, k, v, pos, lo, hi, scale, cap, slopes, out_f32):
     n, nkv = k.shape[:2]
     out, bound = np.zeros((r, nq, hd)), np.zeros((r, nq, hd))
     t = np.arange(n)
+    seen = (t >= lo[:, None]) & (t < hi[:, None])
+    # rows at once where a zero weight takes a value out, else each over the tokens that it sees
+    every = np.isfinite(k).all() and np.isfinite(v).all()
+    parts = [(np.flatnonzero(seen.any(1)), t)] if every else \
+        [(np.array([i]), np.flatnonzero(seen[i])) for i in range(r) if seen[i].any()]
     for h in range(nq):
-        kk, vv = k[:, h // (nq // nkv)], v[:, h // (nq // nkv)]
-        for i in range(r):
-            seen = (t >= lo[i]) & (t < hi[i])
-            if not seen.any():
-                continue
-            ks, vs = kk[seen], vv[seen]
+        for i, ts in parts:
+            kk, vv, see = k[ts, h // (nq // nkv)], v[ts, h // (nq // nkv)], seen[i][:, ts]
+            av = np.abs(vv)
             with np.errstate(all="ignore"):
-                a = scale * (ks @ q[i, h])
-                size = scale * (np.abs(ks) @ np.abs(q[i, h]))
+                a = scale * (q[i, h] @ kk.T)
+                size = scale * (np.abs(q[i, h]) @ np.abs(kk).T)
                 if cap:
                     a = cap * np.tanh(a / cap)
                 if slopes is not None:
-                    far = float(slopes[h]) * np.abs(pos[i] - t[seen])
+                    far = float(slopes[h]) * np.abs(pos[i, None] - ts)
                     a, size = a - far, size + far
                 # only the terms whose weight counts carry their error into the output
-                w = np.exp(a - a.max())
-                p = w / w.sum()
-                out[i, h] = p @ vs
-                e = (hd + 12) * EPS32 * (size + np.abs(a) + np.abs(a.max())) + 2.0 ** -21
-                mean = (p * e).sum()
-                bound[i, h] = 2 * ((p * e) @ np.abs(vs) + mean * (p @ np.abs(vs))) + 2.0 ** -25 * np.abs(vs).sum(0) / w.sum()
+                top = np.where(see, a, -np.inf).max(1, keepdims=True)
+                w = np.where(see, np.exp(a - top), 0.0)
+                total = w.sum(1, keepdims=True)
+                p = w / total
+                out[i, h] = p @ vv
+                e = (hd + 12) * EPS32 * (size + np.abs(a) + np.abs(top)) + 2.0 ** -21
+                e = p * np.where(see, e, 0.0)
+                bound[i, h] = 2 * (e @ av + e.sum(1, keepdims=True) * (p @ av)) + 2.0 ** -25 * (see @ av) / total
                 if not out_f32:
-                    bound[i, h] += EPS16 * (p @ np.abs(vs))
+                    bound[i, h] += EPS16 * (p @ av)
     step = EPS32 if out_f32 else EPS16
     with np.errstate(all="ignore"):
         return out, bound + 2 * step * np.abs(out) + (0 if out_f32 else 2.0 ** -24)

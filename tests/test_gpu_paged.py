@@ -58,6 +58,60 @@ def test_masks(dev, fmt, rows, lens):
         run_case(ia, dev, rng, fmt, 4, 2, 128, rows, lens, first=first, prefix=prefix)
 
 
+@pytest.mark.parametrize("rows,lens", [([1, 4], [400, 77]), ([300], [1700])])
+@pytest.mark.parametrize("cap,scale", [(0.7, 0.3), (3.0, 0.0), (1e4, 0.0), (2e6, 0.1), (50.0, 40.0), (1e-3, 1.0)])
+def test_caps(dev, rows, lens, cap, scale):
+    """Caps that scores never come near, that all of them are far beyond, and both sides of where the polynomial and
+    the exponential share the work."""
+    for f32 in (False, True):
+        announce(f"paged cap={cap} scale={scale} rows={rows} f32={f32}")
+        run_case(ia, dev, np.random.default_rng(3), ia.KV_INT4, 4, 2, 128, rows, lens, cap=cap, scale=scale, out_f32=f32)
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("nq,nkv,hd,rows,lens", [
+    (16, 8, 128, [130], [1000]),                           # two tiles by eight waves
+    (40, 8, 128, [5] * 6, [900, 30, 400, 2000, 33, 700]),  # two tiles by four waves, splits
+    (8, 2, 256, [30, 7], [2000, 300]),
+])
+def test_units_of_two_tiles(dev, fmt, nq, nkv, hd, rows, lens):
+    announce(f"paged units fmt={fmt} {nq}/{nkv}x{hd} rows={rows}")
+    run_case(ia, dev, np.random.default_rng(hd), fmt, nq, nkv, hd, rows, lens, out_f32=fmt == ia.KV_INT8)
+
+
+# Batches with 4096 pages of work and more over their tiles of 128 columns and their kv heads: the workgroups that share
+# their pages.
+SHARED = [
+    (32, 32, 64, [33, 40, 130, 257], [700, 1000, 1500, 1300], {}),
+    (64, 32, 128, [100, 20, 1], [1700, 1500, 60], {"cap": 5.0, "bias": True}),
+    (64, 32, 128, [129, 65], [1301, 1665], {"out_f32": True}),
+    (32, 16, 64, [300], [2601], {"cap": 0.8, "scale": 1.0, "out_f32": True}),
+    (40, 8, 64, [230, 1, 30], [2300, 900, 1000], {"bias": True}),
+    (32, 32, 256, [130, 40], [1500, 1300], {"cap": 30.0}),
+    (32, 32, 256, [150], [2100], {"bias": True, "out_f32": True}),
+]
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("nq,nkv,hd,rows,lens,more", SHARED)
+def test_shared_pages(dev, fmt, nq, nkv, hd, rows, lens, more):
+    announce(f"paged shared fmt={fmt} {nq}/{nkv}x{hd} rows={rows} lens={lens} {more}")
+    run_case(ia, dev, np.random.default_rng(nq + hd + fmt), fmt, nq, nkv, hd, rows, lens, **more)
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_shared_pages_masks(dev, fmt, hd):
+    rows, lens = [140, 45], [1500, 1399]
+    pos = np.concatenate([np.arange(n - r, n) for r, n in zip(rows, lens)])
+    rng = np.random.default_rng(hd)
+    for first, prefix in ((np.where(pos % 3 == 0, pos + 1, np.where(pos % 5 == 0, pos // 64 * 64, 0)), None),
+                          (np.where(pos % 7 == 0, pos // 100 * 100, 40), [1450, 1399]),
+                          (np.where(np.arange(len(pos)) % 50 == 14, 9, 1 << 30), lens)):
+        announce(f"paged shared masks fmt={fmt} hd={hd} first={first[:4]} prefix={prefix}")
+        run_case(ia, dev, rng, fmt, 64, 32, hd, rows, lens, first=first, prefix=prefix, out_f32=hd == 128)
+
+
 @pytest.mark.parametrize("fmt", FMT)
 def test_long_context_is_split(dev, fmt):
     """Splits over a long axis and their join, beside short rows in one batch."""
@@ -77,16 +131,16 @@ def _setup(dev, fmt, nq, nkv, hd, rows, lens, seed=0, edit=None):
 
 
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
-@pytest.mark.parametrize("rows,lens", [([1, 3], [70, 80]), ([100], [150])])
-def test_values_that_a_row_does_not_see_do_not_reach_it(dev, rows, lens, value):
+@pytest.mark.parametrize("rows,lens,nkv", [([1, 3], [70, 80], 2), ([100], [150], 2), ([70, 66], [900, 1500], 32)])
+def test_values_that_a_row_does_not_see_do_not_reach_it(dev, rows, lens, nkv, value):
     """Infinities and NaN in the K and V of positions that some rows see and others do not: the rows that do not see
     them give what they give without them, the others what the formula gives."""
-    fmt, nq, nkv, hd = ia.KV_FP16, 4, 2, 128
+    fmt, nq, hd = ia.KV_FP16, 2 * nkv, 128
     bad = [(s, lens[s] - rows[s] // 2 - 1, v) for s in range(len(rows)) for v in (0, 1)] + [(0, 5, 1), (0, 6, 0)]
 
     def edit(cache, table):
         for s, t, v in bad:
-            cache.pool[table[s, t // 32], 1, v].view(np.float16)[pr.element(fmt, hd, v)[t % 32, 3::16]] = value
+            cache.pool[table[s, t // 32], nkv - 1, v].view(np.float16)[pr.element(fmt, hd, v)[t % 32, 3::16]] = value
 
     pos = np.concatenate([np.arange(n - r, n) for r, n in zip(rows, lens)])
     first = np.full(len(pos), 8)
@@ -103,14 +157,49 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(dev, rows, lens, value):
                      for m in range(len(pos))])
     same = ~sees.any(1)
     assert (np.abs(got - want)[same] <= tol[same]).all()
-    assert (np.abs(got - want)[:, :2] <= tol[:, :2]).all()   # the other kv head's queries
-    hurt = ~np.isfinite(got[:, 2:])
+    assert (np.abs(got - want)[:, :-2] <= tol[:, :-2]).all()   # the other kv heads' queries
+    hurt = ~np.isfinite(got[:, -2:])
     only_v = sees[:, 1] & ~sees[:, 0]
     dims = np.zeros(hd, bool)
     dims[3::16] = True
     assert hurt[sees[:, 1]][:, :, dims].all() and not hurt[only_v][:, :, ~dims].any()
     if np.isnan(value):
-        assert np.isnan(got[sees[:, 0], 2:]).all()
+        assert np.isnan(got[sees[:, 0], -2:]).all()
+    plan.close()
+
+
+@pytest.mark.parametrize("fmt", [ia.KV_INT8, ia.KV_INT4])
+@pytest.mark.parametrize("rows,lens,nkv", [([1, 3], [70, 80], 2), ([100], [150], 2), ([70, 66], [900, 1500], 32)])
+def test_quantized_rows_without_a_scale(dev, fmt, rows, lens, nkv):
+    """Rows that were stored with a NaN (their scale is NaN) reach only the rows that see them: K the whole head, V its
+    group's dims."""
+    nq, hd = 2 * nkv, 128
+    rng = np.random.default_rng(7)
+    n_pages, table, pos = pr.batch(rng, rows, lens)
+    M, plan = len(pos), ia.Paged(dev, fmt, nq, nkv, hd, n_pages)
+    cache = pr.Cache(fmt, nkv, hd, n_pages, rng)
+    pool, q = dev.upload(cache.pool), f16(rng, M, nq, hd)
+    k, v = f16(rng, M, nkv, hd), f16(rng, M, nkv, hd)
+    bad_k, bad_v = M // 2, M - 1 if M < 5 else 2 * M // 3   # batch rows
+    kn, vn = k.copy(), v.copy()
+    kn[bad_k, 1, 9] = np.nan
+    vn[bad_v, 0, 70] = np.inf
+    plan.set(rows, lens, table)
+    qd, kd, vd, out = dev.upload(q), dev.upload(kn), dev.upload(vn), dev.alloc(q.size * 4)
+    announce(f"paged quantized NaN fmt={fmt} rows={rows}")
+    plan.append(pool.p, kd.p, vd.p)
+    plan.attention(pool.p, qd.p, out.p, out_f32=True)
+    got = dev.download(out, np.float32, q.shape).astype(np.float64)
+    seq = np.repeat(np.arange(len(rows)), rows)
+    for m in range(M):
+        cache.append(table[seq[m]], pos[m], k[m].astype(np.float32), v[m].astype(np.float32))
+    want, tol = pr.expect(cache, rows, lens, table, q, out_f32=True)
+    sees = lambda b: (seq == seq[b]) & (pos >= pos[b])  # noqa: E731
+    hurt = np.zeros(q.shape, bool)
+    hurt[sees(bad_k), 2:4] = True
+    hurt[sees(bad_v), :2, slice(64, 128) if fmt == ia.KV_INT4 else slice(0, 128)] = True
+    assert np.isnan(got[hurt]).all()
+    assert (np.abs(got - want)[~hurt] <= tol[~hurt]).all()
     plan.close()
 
 

@@ -7,7 +7,7 @@ import pytest
 from tests.hipemu import runner
 from tests.test_hipemu import emu_lib  # noqa: F401
 
-ORDER = ["paged_chunks", "paged_rows", "paged_refusals"]
+ORDER = ["paged_shared_int8", "paged_shared_int4", "paged_shared_fp16", "paged_chunks", "paged_rows", "paged_refusals"]
 
 
 @pytest.fixture(scope="module")
