@@ -69,14 +69,31 @@ def test_caps(dev, rows, lens, cap, scale):
 
 
 @pytest.mark.parametrize("fmt", FMT)
-@pytest.mark.parametrize("nq,nkv,hd,rows,lens", [
-    (16, 8, 128, [130], [1000]),                           # two tiles by eight waves
-    (40, 8, 128, [5] * 6, [900, 30, 400, 2000, 33, 700]),  # two tiles by four waves, splits
-    (8, 2, 256, [30, 7], [2000, 300]),
+@pytest.mark.parametrize("nq,nkv,hd,rows,lens,more", [
+    # two tiles by eight waves: 13 to 24 pages, or tiles of like lengths that the CUs hold at once
+    (16, 8, 128, [130, 20], [500, 300], {}),
+    (4, 2, 128, [99], [757], {"cap": 7.0, "bias": True, "out_f32": True}),
+    (32, 32, 128, [250], [1000], {"out_f32": True}),
+    (32, 32, 128, [249], [1000], {"prefix": [970], "bias": True}),
+    # by four, with splits
+    (16, 8, 128, [130], [1000], {}),
+    (40, 8, 128, [5] * 6, [900, 30, 400, 2000, 33, 700], {"out_f32": True}),
+    (8, 2, 256, [30, 7], [2000, 300], {}),
 ])
-def test_units_of_two_tiles(dev, fmt, nq, nkv, hd, rows, lens):
-    announce(f"paged units fmt={fmt} {nq}/{nkv}x{hd} rows={rows}")
-    run_case(ia, dev, np.random.default_rng(hd), fmt, nq, nkv, hd, rows, lens, out_f32=fmt == ia.KV_INT8)
+def test_units_of_two_tiles(dev, fmt, nq, nkv, hd, rows, lens, more):
+    announce(f"paged units fmt={fmt} {nq}/{nkv}x{hd} rows={rows} {more}")
+    run_case(ia, dev, np.random.default_rng(hd), fmt, nq, nkv, hd, rows, lens, **more)
+
+
+@pytest.mark.parametrize("fmt", FMT)
+def test_units_of_two_tiles_masks(dev, fmt):
+    pos = np.arange(370, 500)
+    rng = np.random.default_rng(fmt)
+    for first, prefix in ((np.where(pos % 3 == 0, pos + 1, np.where(pos % 5 == 0, pos // 64 * 64, 0)), None),
+                          (np.where(pos % 7 == 0, pos // 100 * 100, 3), [450]),
+                          (np.where(pos % 50 == 14, 9, 1 << 30), [500])):
+        announce(f"paged units masks fmt={fmt} first={first[:4]} prefix={prefix}")
+        run_case(ia, dev, rng, fmt, 16, 8, 128, [130], [500], first=first, prefix=prefix, out_f32=prefix is None)
 
 
 # Batches with 4096 pages of work and more over their tiles of 128 columns and their kv heads: the workgroups that share
@@ -131,7 +148,7 @@ def _setup(dev, fmt, nq, nkv, hd, rows, lens, seed=0, edit=None):
 
 
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
-@pytest.mark.parametrize("rows,lens,nkv", [([1, 3], [70, 80], 2), ([100], [150], 2), ([70, 66], [900, 1500], 32)])
+@pytest.mark.parametrize("rows,lens,nkv", [([1, 3], [70, 80], 2), ([100], [150], 2), ([130], [500], 8), ([70, 66], [900, 1500], 32)])
 def test_values_that_a_row_does_not_see_do_not_reach_it(dev, rows, lens, nkv, value):
     """Infinities and NaN in the K and V of positions that some rows see and others do not: the rows that do not see
     them give what they give without them, the others what the formula gives."""
@@ -169,7 +186,7 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(dev, rows, lens, nkv, va
 
 
 @pytest.mark.parametrize("fmt", [ia.KV_INT8, ia.KV_INT4])
-@pytest.mark.parametrize("rows,lens,nkv", [([1, 3], [70, 80], 2), ([100], [150], 2), ([70, 66], [900, 1500], 32)])
+@pytest.mark.parametrize("rows,lens,nkv", [([1, 3], [70, 80], 2), ([100], [150], 2), ([130], [500], 8), ([70, 66], [900, 1500], 32)])
 def test_quantized_rows_without_a_scale(dev, fmt, rows, lens, nkv):
     """Rows that were stored with a NaN (their scale is NaN) reach only the rows that see them: K the whole head, V its
     group's dims."""
