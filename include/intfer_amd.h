@@ -304,10 +304,10 @@ int ifr_quant_gemm_ga(ifr_ctx* ctx, const ifr_dlinear* w, const int8_t* a_d, con
  * ---------------------------------------------------------------------- */
 enum {
   IFR_KV_FP16 = 0, /* fp16 */
-  IFR_KV_INT8 = 1, /* s = fp16(max|x| / 127) per (token, kv head), codes half
-                    * away from zero; a code stands for fp16(c s) */
-  IFR_KV_INT4 = 2  /* z = fp16(min), s = fp16((max - min) / 15) per (token, kv
-                    * head, 64 dims), codes rint((x - z) (1 / s)) in 0 .. 15;
+  IFR_KV_INT8 = 1, /* s = fp16(max|x| (1 / 127)) per (token, kv head), codes
+                    * half away from zero; a code stands for fp16(c s) */
+  IFR_KV_INT4 = 2  /* z = fp16(min), s = fp16((max - min) (1 / 15)) per (token,
+                    * kv head, 64 dims), codes rint((x - z) (1 / s)) in 0 .. 15;
                     * a code stands for fp16(c s + z), rounded once */
 };
 /* A group of an 8- or 4-bit row that holds a NaN or an infinity reads back

@@ -6,9 +6,12 @@
 // with every product and the sum rounded to fp32.  K is stored from that fp32
 // value, so the only rounding after it is the format's own:
 //   fp16  fp16(x)
-//   int8  s = fp16(max|x| / 127) per (token, head), c = half-away(x * (1 / s))
-//   int4  z = fp16(min), s = fp16((max - min) / 15) per (token, head, 64 dims),
-//         c = rint((x - z) * (1 / s)) in 0 .. 15; it stands for fp16(c s + z)
+//   int8  s = fp16(max|x| * (1 / 127)) per (token, head),
+//         c = half-away(x * (1 / s))
+//   int4  z = fp16(min), s = fp16((max - min) * (1 / 15)) per (token, head, 64
+//         dims), c = rint((x - z) * (1 / s)) in 0 .. 15; it stands for
+//         fp16(c s + z)
+// (reciprocals and products rounded to fp32 each).
 // A group that holds a NaN or an infinity gets a NaN scale and reads back as
 // NaN; the codes of a group whose scale rounds to zero are zero.  A scale whose
 // largest code would round to infinity is the next smaller one (int8: 515.5 at
@@ -54,7 +57,7 @@ __device__ __forceinline__ void quantize8(const float (&x)[8], uint32_t (&code)[
 #pragma unroll
     for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(x[e]));
     a = group_max<LPT>(a);
-    scale = bad ? (uint16_t)0x7E00u : ifrd::f2h(fminf(a / 127.0f, 515.5f));
+    scale = bad ? (uint16_t)0x7E00u : ifrd::f2h(fminf(a * (1.0f / 127.0f), 515.5f));
     const float s = ifrd::h2f(scale);
     const float inv = s > 0.0f && !bad ? 1.0f / s : 0.0f;
     code[0] = code[1] = 0u;
@@ -75,7 +78,7 @@ __device__ __forceinline__ void quantize8(const float (&x)[8], uint32_t (&code)[
     lo = -group_max<8>(-lo);
     lo = fminf(fmaxf(lo, -kMaxHalf), kMaxHalf);  // (a rotated value can pass fp16's range)
     hi = fminf(fmaxf(hi, -kMaxHalf), kMaxHalf);
-    scale = ifrd::f2h((hi - lo) / 15.0f);
+    scale = ifrd::f2h((hi - lo) * (1.0f / 15.0f));
     zero = ifrd::f2h(lo);
     if (15.0f * ifrd::h2f(scale) + ifrd::h2f(zero) >= 65520.0f) scale -= 1;  // code 15 would round to infinity
     if (bad) {

@@ -77,7 +77,7 @@ def quantize(x, fmt):
             return x.astype(np.float16), None, None
         if fmt == INT8:
             bad = ~np.isfinite(x).all(-1, keepdims=True)
-            s = np.where(bad, np.float32(0), np.abs(x)).max(-1, keepdims=True) / np.float32(127)
+            s = np.where(bad, np.float32(0), np.abs(x)).max(-1, keepdims=True) * (one / np.float32(127))
             s = np.minimum(s, np.float32(515.5)).astype(np.float16)  # 127 * 516 would round to infinity
             f = s.astype(np.float32)
             y = np.where(bad, np.float32(0), x) * np.where(f > 0, one / f, np.float32(0))
@@ -89,7 +89,7 @@ def quantize(x, fmt):
         bad = ~np.isfinite(g).all(-1, keepdims=True)
         g = np.where(bad, np.float32(0), g)
         lo, hi = (np.clip(f(-1, keepdims=True), -65504, 65504).astype(np.float32) for f in (g.min, g.max))
-        z, s = lo.astype(np.float16), ((hi - lo) / np.float32(15)).astype(np.float16)
+        z, s = lo.astype(np.float16), ((hi - lo) * (one / np.float32(15))).astype(np.float16)
         over = 15 * s.astype(np.float64) + z.astype(np.float64) >= 65520  # code 15 would round to infinity
         s = np.where(over, (s.view(np.uint16) - 1).astype(np.uint16).view(np.float16), s)
         f = s.astype(np.float32)
