@@ -105,15 +105,16 @@ struct PagedAttnArgs {
   float* part_ml;           // [columns][2]
 };
 // narrow units: up to 16 * tiles columns (tiles 1 or 2) by workgroups of 4
-// waves, or 8 (two tiles, heads of 128); wide units: up to kPgWide columns.
-constexpr int kPgWide = 128;
+// waves, or 8 (two tiles, heads of 128); wide units: up to kPgWide columns, heads
+// of up to kPgWideDim.
+constexpr int kPgWide = 128, kPgWideDim = 128;
 // Waves a SIMD that a narrow kernel's registers leave (o, q and the raw page),
 // and workgroups a CU of a wide one.
 constexpr int paged_narrow_waves(int fmt, int hd, int nt) {
   return fmt == IFR_KV_FP16 && hd >= 128 ? (hd == 128 ? 2 : 1)
                                          : hd * nt <= 64 ? 4 : hd * nt <= 128 ? 3 : hd * nt <= 256 ? 2 : 1;
 }
-constexpr int paged_wide_groups(int hd) { return hd == 256 ? 1 : 2; }
+constexpr int kPgWideGroups = 2;
 hipError_t launch_paged_narrow(const PagedAttnArgs& a, const PagedPool& kv, int tiles, int waves, hipStream_t st);
 hipError_t launch_paged_wide(const PagedAttnArgs& a, const PagedPool& kv, hipStream_t st);
 hipError_t launch_paged_join(const PagedJoin* joins, int n, const PagedAttnArgs& a, const PagedPool& kv,

@@ -50,8 +50,17 @@ constexpr int kWhole = 3;
 // start, and narrow units, four times as many, win although they turn the pages
 // into fp16 four times (16/8 heads of 128, int4, us narrow / wide: 64 rows on 500
 // tokens 10.9 / 16.0, 256 on 2000, 2112 pages, 23.0 / 27.2, 512 on 2000, 4544,
-// 33.8 / 34.2, 256 on 8000, 8128, 45.8 / 43.1).
+// 33.8 / 34.2, 256 on 8000, 8128, 45.8 / 43.1).  Over fp16 pages, which need no
+// turning, they have to fill the CUs besides (us narrow / wide: 4000 causal rows,
+// 504 tiles, 101 / 109; 8000, 1000 tiles, 349 / 311; 4000 of 32/4 heads 198 / 164).
 constexpr int64_t kWidePages = 16 * kCUs;
+// A batch with units of two tiles takes its sequences of one tile in such units
+// too, if these have few pages: their second tile is idle, but they run beside
+// the others and not in a launch before them (16/8 heads of 128, int4, us two
+// launches / one: 24 decode rows on 1000 tokens and a chunk of 512 32.4 / 28.2, 8
+// on 1300 and 72 24.3 / 14.5, 8 on 4000 and 256 35.3 / 28.8, 64 on 1000 and 64,
+// 20 thousand pages, 33.4 / 34.2).
+constexpr int64_t kMergePages = 64 * kCUs;
 // Two-tile units of heads of 128 leave a CU eight waves.  One workgroup of all
 // of them takes whole tiles where two of four would need splits and a join: if
 // the CUs hold all tiles at once and the longest is not far over the mean, or is
@@ -226,7 +235,9 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
   for (int s = 0; s < S; ++s)
     if ((int64_t)b->rows[s] * G > kWidth[1]) cut(kWide, s, wide);
   for (const Tile& t : wide) wide_pages += (int64_t)(t.p1 - t.p0) * c.n_kv;
-  const bool use_wide = wide_pages >= kWidePages;
+  constexpr int64_t wide_slots = (int64_t)kCUs * ifrk::kPgWideGroups;
+  const bool use_wide = c.head_dim <= ifrk::kPgWideDim && wide_pages >= kWidePages &&
+                        (c.format != IFR_KV_FP16 || (int64_t)wide.size() * c.n_kv >= wide_slots);
   if (use_wide) tiles = wide;
   for (int s = 0; s < S; ++s) {
     const int64_t n = (int64_t)b->rows[s] * G;
@@ -240,6 +251,14 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
     pages[t.kind] += t.p1 - t.p0;
     most[t.kind] = std::max<int64_t>(most[t.kind], t.p1 - t.p0);
     ++n_tiles[t.kind];
+  }
+  if (n_tiles[1] > 0 && pages[0] * c.n_kv < kMergePages) {
+    for (Tile& t : tiles)
+      if (t.kind == 0) t.kind = 1;
+    pages[1] += pages[0];
+    most[1] = std::max(most[0], most[1]);
+    n_tiles[1] += n_tiles[0];
+    pages[0] = most[0] = n_tiles[0] = 0;
   }
   const int64_t eight = kCUs * ifrk::paged_narrow_waves(c.format, c.head_dim, 2) / 2;  // workgroups at once
   if (c.head_dim == 128 && n_tiles[1] * c.n_kv <= eight &&
@@ -256,7 +275,7 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
   // share of a workgroup.
   int wants[kKinds], grains[kKinds];
   for (int k = 0; k < kKinds; ++k) {
-    const int64_t slots = k == kWide ? kCUs * ifrk::paged_wide_groups(c.head_dim)
+    const int64_t slots = k == kWide ? wide_slots
                                      : kCUs * ifrk::paged_narrow_waves(c.format, c.head_dim, kTiles[k]) * 4 / kWaves[k];
     const int g = grains[k] = k == kWide ? kWideGrain : kWaves[k], least = k == kWide ? kWideMin : kWaves[k];
     const auto grain = [&](int64_t n) { return (int)std::max<int64_t>(least, (n + g - 1) / g * g); };
@@ -271,6 +290,10 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
         if (units * c.n_kv <= slots) hi = mid;
         else lo = mid + g;
       }
+    // A causal prompt's tiles differ in length up to its own.  Where they all run
+    // at once unsplit, those of more than three quarters of the longest are split
+    // (4000 rows over 4-bit pages, 16/8 heads of 128, 129.9 -> 113.0 us).
+    if (k == kWide && lo >= most[k] && 5 * share <= 3 * most[k]) lo = grain(most[k] * 3 / 4);
     wants[k] = lo;
   }
   std::vector<ifrk::PagedUnit> units[kKinds];
@@ -281,23 +304,35 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
     const int cuts = t.kind != kWide && np <= kWhole * grains[t.kind] ? 1 : std::max(1, (np + want - 1) / want);
     const int g = grains[t.kind], step = cuts == 1 ? std::max(np, 1) : ((np + cuts - 1) / cuts + g - 1) / g * g;
     const int ns = std::max(1, (np + step - 1) / step);
-    for (int h = 0; h < c.n_kv; ++h) {
-      const int64_t base = cols;
-      for (int s = 0; s < ns; ++s) {
+    // (heads inside splits: with 8 kv heads a head's units run on one XCD)
+    const int64_t base = cols;
+    for (int s = 0; s < ns; ++s)
+      for (int h = 0; h < c.n_kv; ++h) {
         const int p0 = t.p0 + s * step, p1 = std::min(t.p1, p0 + step);
-        units[t.kind].push_back({row0[t.seq], h, t.col0, t.ncol, tab[t.seq], p0, p1, ns == 1 ? -1 : (int)cols});
-        if (ns > 1) cols += t.ncol;
+        const int64_t part = base + ((int64_t)h * ns + s) * t.ncol;
+        units[t.kind].push_back({row0[t.seq], h, t.col0, t.ncol, tab[t.seq], p0, p1, ns == 1 ? -1 : (int)part});
       }
+    if (ns > 1) {
+      cols += (int64_t)c.n_kv * ns * t.ncol;
       if (cols > kMaxTokens) return fail(IFR_EINVAL, "too many partial columns");
-      if (ns > 1)
+      for (int h = 0; h < c.n_kv; ++h)
         for (int i = 0, n = 1024 / c.head_dim; i < t.ncol; i += n)
-          joins.push_back({row0[t.seq], h, t.col0 + i, std::min(n, t.ncol - i), (int)base + i, t.ncol, ns, 0});
+          joins.push_back({row0[t.seq], h, t.col0 + i, std::min(n, t.ncol - i), (int)(base + (int64_t)h * ns * t.ncol) + i, t.ncol, ns, 0});
     }
   }
   // the longest first, for short ones to fill the end
   for (auto& u : units)
     std::stable_sort(u.begin(), u.end(),
                      [](const ifrk::PagedUnit& x, const ifrk::PagedUnit& y) { return x.p1 - x.p0 > y.p1 - y.p0; });
+  // Of wide units a CU takes one of the first 256 and one of the next: these in
+  // rising order put a short one beside a long one (8000 rows capped, in four
+  // documents, 175 -> 166 us; 2 x 1000 on 2777 63.5 -> 60.9).  Eight at a time,
+  // the heads' XCDs as they were.
+  if (auto& u = units[kWide]; u.size() > (size_t)kCUs) {
+    const size_t n = std::min<size_t>(u.size() - kCUs, kCUs) / 8;
+    for (size_t i = 0; i < n / 2; ++i)
+      std::swap_ranges(u.begin() + kCUs + 8 * i, u.begin() + kCUs + 8 * (i + 1), u.begin() + kCUs + 8 * (n - 1 - i));
+  }
   size_t at = 0;
   auto room = [&](size_t bytes) {
     const size_t o = at;

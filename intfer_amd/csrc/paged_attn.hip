@@ -346,9 +346,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedJoin* joins,
 //
 // HL: P enters the second product as an fp16 high + low pair (22 bits), for
 // outputs in fp32.  An fp16 output takes P rounded to fp16, which is off like
-// the output's own rounding and saves 5 % (64 rows of 2048 int4 tokens 60.2 ->
-// 57.3 us, 16 of 32000 160.6 -> 152.3).  Bound by its VALU work at 4 bits:
-// 13 operations turn a dword of codes into 8 values.  (Two K buffers and both
+// the output's own rounding and saves 5 % (64 rows of 2048 int4 tokens, with
+// the first plan, 60.2 -> 57.3 us, 16 of 32000 160.6 -> 152.3).  Bound by its VALU work at 4 bits:
+// 13 operations turn a dword of codes into 8 values; the 64 rows take 40 to 44 us
+// where their bytes would take 32, the 16 rows 117 to 126 of 104.  (Two K buffers and both
 // steps unrolled spilled at 192 VGPRs: 142.8 and 467 us.)
 template <int HD, int FMT, int NT, int NW, bool HL>
 __global__ __launch_bounds__(64 * NW, paged_narrow_waves(FMT, HD, NT)) void paged_narrow_kernel(PagedAttnArgs a, PagedPool kv) {
@@ -638,6 +639,12 @@ __global__ __launch_bounds__(64 * NW, paged_narrow_waves(FMT, HD, NT)) void page
 // 16-byte runs of a dim block (K) or of 16 dims (V) are rotated against each
 // other by an exclusive or, which spreads both the quantized formats' stores
 // and the reads over the banks.
+//
+// Bound by its matrix products and the softmax's VALU work between them: 8000
+// causal fp16 rows of 16/8 heads of 128 take 311 us (840 TFLOP/s), over 4-bit
+// pages 342; two-tile units 349 and 468.  With a cap and four documents 167.
+// Heads of 256 leave LDS for one such workgroup a CU, and two-tile units win:
+// 4000 causal fp16 rows of 8/2 heads 244 us here, 114 there, 4-bit 289 and 166.
 __device__ __forceinline__ int wide_tok(int rho) {
   return 8 * (rho >> 4) + 4 * ((rho >> 2) & 1) + 16 * ((rho >> 3) & 1) + (rho & 3);
 }
@@ -649,8 +656,9 @@ template <int HD>
 __device__ __forceinline__ int v_run(int g, int d) { return g * HD + (d ^ ((d >> 4) & 15)); }
 
 template <int HD, int FMT, bool HL>
-__global__ __launch_bounds__(256, paged_wide_groups(HD)) void paged_wide_kernel(PagedAttnArgs a, PagedPool kv) {
-  constexpr int NP = HD == 256 ? 1 : 2;
+__global__ __launch_bounds__(256, kPgWideGroups) void paged_wide_kernel(PagedAttnArgs a, PagedPool kv) {
+  constexpr int NP = 2;
+  static_assert(HD <= kPgWideDim, "LDS for two workgroups a CU");
   constexpr int I = HD / 32, N = HD / 16, U = HD / kPgGroup, KS = HD / 16, D = HD / 32;
   constexpr int RUNS = 4 * HD;  // 16-byte runs of a page's K (or V) in LDS
   constexpr size_t kPart = paged_part(FMT, HD);
@@ -930,10 +938,14 @@ hipError_t narrow_fmt(const PagedAttnArgs& a, const PagedPool& kv, int tiles, in
 
 template <int HD, int FMT>
 hipError_t wide_fmt(const PagedAttnArgs& a, const PagedPool& kv, hipStream_t st) {
-  const dim3 grid(a.n_units), block(256);
-  if (a.out_f32) hipLaunchKernelGGL((paged_wide_kernel<HD, FMT, true>), grid, block, 0, st, a, kv);
-  else hipLaunchKernelGGL((paged_wide_kernel<HD, FMT, false>), grid, block, 0, st, a, kv);
-  return hipGetLastError();
+  if constexpr (HD > kPgWideDim) {
+    return hipErrorInvalidValue;
+  } else {
+    const dim3 grid(a.n_units), block(256);
+    if (a.out_f32) hipLaunchKernelGGL((paged_wide_kernel<HD, FMT, true>), grid, block, 0, st, a, kv);
+    else hipLaunchKernelGGL((paged_wide_kernel<HD, FMT, false>), grid, block, 0, st, a, kv);
+    return hipGetLastError();
+  }
 }
 
 }  // namespace

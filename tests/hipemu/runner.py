@@ -784,30 +784,30 @@ def paged_chunks():
     case(2, 2, 1, 64, [50], [140], first=pos // 3, prefix=[130], rotary=16)
 
 
-def _paged_shared(fmt, hd, **more):
+def _paged_shared(fmt, n, hd, rows, lens, **more):
     import intfer_amd as ia
     from tests.paged_check import run_case
-    run_case(ia, ia.Device(0), np.random.default_rng(5), fmt, 32, 32, hd, [33, 130], [700, 1900], say=say, **more)
+    run_case(ia, ia.Device(0), np.random.default_rng(5), fmt, n, n, hd, rows, lens, say=say, **more)
 
 
 @scenario
 def paged_shared_fp16():
     """Chunks with enough pages of work for the workgroups of 128 columns that share their pages; documents, and rows
     that see nothing."""
-    pos = np.concatenate([np.arange(667, 700), np.arange(1770, 1900)])
-    _paged_shared(0, 64, first=np.where(pos % 3 == 0, pos // 29 * 29, np.where(pos % 5 == 0, pos + 1, 3)), out_f32=True)
+    pos = np.concatenate([np.arange(170, 300), np.arange(129), np.arange(170, 300), np.arange(250, 390)])
+    _paged_shared(0, 64, 64, [130, 129, 130, 140], [300, 129, 300, 390], first=np.where(pos % 3 == 0, pos // 29 * 29, np.where(pos % 5 == 0, pos + 1, 3)), out_f32=True)
 
 
 @scenario
 def paged_shared_int8():
     """The same over int8 pages: a cap, a prefix."""
-    _paged_shared(1, 128, cap=4.0, prefix=[690, 5])
+    _paged_shared(1, 32, 128, [33, 130], [700, 1900], cap=4.0, prefix=[690, 5])
 
 
 @scenario
 def paged_shared_int4():
     """The same over 4-bit pages: cap and bias at once."""
-    _paged_shared(2, 64, cap=9.0, bias=True, out_f32=True)
+    _paged_shared(2, 32, 64, [33, 130], [700, 1900], cap=9.0, bias=True, out_f32=True)
 
 
 @scenario

@@ -96,15 +96,19 @@ def test_units_of_two_tiles_masks(dev, fmt):
         run_case(ia, dev, rng, fmt, 16, 8, 128, [130], [500], first=first, prefix=prefix, out_f32=prefix is None)
 
 
-# Batches with 4096 pages of work and more over their tiles of 128 columns and their kv heads: the workgroups that share
-# their pages.
+# Batches with 4096 pages of work and more over their tiles of 128 columns and their kv heads (over fp16 pages 512 tiles
+# and more as well): the workgroups that share their pages.
 SHARED = [
+    (64, 64, 64, [129, 130, 200, 140], [600, 500, 420, 700], {"cap": 12.0, "out_f32": True}),
+    (64, 64, 128, [257, 300, 140], [257, 500, 410], {"bias": True}),
     (32, 32, 64, [33, 40, 130, 257], [700, 1000, 1500, 1300], {}),
     (64, 32, 128, [100, 20, 1], [1700, 1500, 60], {"cap": 5.0, "bias": True}),
     (64, 32, 128, [129, 65], [1301, 1665], {"out_f32": True}),
     (32, 16, 64, [300], [2601], {"cap": 0.8, "scale": 1.0, "out_f32": True}),
     (40, 8, 64, [230, 1, 30], [2300, 900, 1000], {"bias": True}),
-    (32, 32, 256, [130, 40], [1500, 1300], {"cap": 30.0}),
+    (64, 32, 128, [150, 290], [1700, 1600], {"cap": 30.0, "out_f32": True}),
+    (32, 4, 64, [530], [2500], {"cap": 30.0}),
+    (32, 32, 256, [130, 40], [1500, 1300], {"cap": 30.0}),  # (two-tile units of many columns)
     (32, 32, 256, [150], [2100], {"bias": True, "out_f32": True}),
 ]
 
@@ -117,16 +121,16 @@ def test_shared_pages(dev, fmt, nq, nkv, hd, rows, lens, more):
 
 
 @pytest.mark.parametrize("fmt", FMT)
-@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("hd", [64, 128])
 def test_shared_pages_masks(dev, fmt, hd):
-    rows, lens = [140, 45], [1500, 1399]
+    rows, lens = [270, 250], [500, 600]
     pos = np.concatenate([np.arange(n - r, n) for r, n in zip(rows, lens)])
     rng = np.random.default_rng(hd)
     for first, prefix in ((np.where(pos % 3 == 0, pos + 1, np.where(pos % 5 == 0, pos // 64 * 64, 0)), None),
-                          (np.where(pos % 7 == 0, pos // 100 * 100, 40), [1450, 1399]),
+                          (np.where(pos % 7 == 0, pos // 100 * 100, 40), [450, 599]),
                           (np.where(np.arange(len(pos)) % 50 == 14, 9, 1 << 30), lens)):
         announce(f"paged shared masks fmt={fmt} hd={hd} first={first[:4]} prefix={prefix}")
-        run_case(ia, dev, rng, fmt, 64, 32, hd, rows, lens, first=first, prefix=prefix, out_f32=hd == 128)
+        run_case(ia, dev, rng, fmt, 128, 64, hd, rows, lens, first=first, prefix=prefix, out_f32=hd == 128)
 
 
 @pytest.mark.parametrize("fmt", FMT)
@@ -148,7 +152,7 @@ def _setup(dev, fmt, nq, nkv, hd, rows, lens, seed=0, edit=None):
 
 
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
-@pytest.mark.parametrize("rows,lens,nkv", [([1, 3], [70, 80], 2), ([100], [150], 2), ([130], [500], 8), ([70, 66], [900, 1500], 32)])
+@pytest.mark.parametrize("rows,lens,nkv", [([1, 3], [70, 80], 2), ([100], [150], 2), ([130], [500], 8), ([260, 260], [400, 500], 64)])
 def test_values_that_a_row_does_not_see_do_not_reach_it(dev, rows, lens, nkv, value):
     """Infinities and NaN in the K and V of positions that some rows see and others do not: the rows that do not see
     them give what they give without them, the others what the formula gives."""
@@ -186,7 +190,7 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(dev, rows, lens, nkv, va
 
 
 @pytest.mark.parametrize("fmt", [ia.KV_INT8, ia.KV_INT4])
-@pytest.mark.parametrize("rows,lens,nkv", [([1, 3], [70, 80], 2), ([100], [150], 2), ([130], [500], 8), ([70, 66], [900, 1500], 32)])
+@pytest.mark.parametrize("rows,lens,nkv", [([1, 3], [70, 80], 2), ([100], [150], 2), ([130], [500], 8), ([260, 260], [400, 500], 64)])
 def test_quantized_rows_without_a_scale(dev, fmt, rows, lens, nkv):
     """Rows that were stored with a NaN (their scale is NaN) reach only the rows that see them: K the whole head, V its
     group's dims."""
