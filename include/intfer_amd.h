@@ -312,7 +312,8 @@ enum {
 };
 /* A group of an 8- or 4-bit row that holds a NaN or an infinity reads back
  * as NaN (its scale is NaN); of any other the scale is small enough for all
- * codes to stand for finite values, which the attention relies on.  A page holds 32 tokens: per kv head one block
+ * codes to stand for finite values, which the attention relies on.  A page
+ * holds 32 tokens: per kv head one block
  *   [K codes][K scales][V codes][V scales],
  * heads in order, pages back to back, ifr_paged_bytes in all.  The element
  * order inside a block is the order of the matrix instructions that read it,
@@ -373,9 +374,9 @@ int ifr_paged_set(ifr_paged* p, const ifr_paged_batch* b);
  * back to back inside a row; 16-byte aligned, strides a multiple of 8 (slices
  * of a fused QKV output qualify).  The rotation is rotate-half (rope,
  * main.cpp:365-373) over the first `rotary` dims with the fp32 tables
- * cos_d, sin_d [max_pos][rotary / 2] (16-byte aligned), in fp32; K is stored from the fp32
- * result.  Q is rotated into q_out_d, which is q_d itself (same stride) or
- * overlaps nothing; both NULL: no Q. */
+ * cos_d, sin_d [max_pos][rotary / 2] (16-byte aligned), in fp32; K is stored
+ * from the fp32 result.  Q is rotated into q_out_d, which is q_d itself (same
+ * stride) or overlaps nothing; both NULL: no Q. */
 typedef struct ifr_paged_rows {
   const uint16_t* k_d; /* [M][n_kv][head_dim] */
   const uint16_t* v_d;
@@ -393,7 +394,10 @@ int ifr_paged_append(ifr_paged* p, void* pool_d, const ifr_paged_rows* r);
 /* Attention of the batch's rows, whose K and V are in the pages already.  The
  * score of position t is a = scale q.k, then cap tanh(a / cap) where softcap
  * is set, then minus slopes[head] * |pos - t| where slopes are; softmax over
- * the positions that the row sees. */
+ * the positions that the row sees.  Sums and statistics are fp32; for an fp32
+ * output the weights enter the second product with 22 bits, for an fp16 output
+ * with 11.  The same batch gives the same bits; how its sequences are split
+ * depends on the whole batch, and with it a row's last bits. */
 typedef struct ifr_paged_query {
   const uint16_t* q_d;  /* fp16 [M][n_heads][head_dim] */
   int64_t q_stride;     /* elements, a multiple of 8 */
