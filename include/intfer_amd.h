@@ -404,8 +404,8 @@ typedef struct ifr_paged_query {
   void* out_d;          /* fp16, or fp32 for ifr_act_quant; not q_d */
   int64_t out_stride;   /* elements, a multiple of 16 bytes */
   int32_t out_f32;      /* 0: fp16, 1: fp32 */
-  float scale;          /* 0: 1 / sqrt(head_dim) */
-  float softcap;        /* 0: none */
+  float scale;          /* 0: 1 / sqrt(head_dim); up to 1e30 */
+  float softcap;        /* 0: none; it and scale / softcap up to 1e30 */
   const float* slopes_d; /* fp32 [n_heads] or NULL */
 } ifr_paged_query;
 int ifr_paged_attention(ifr_paged* p, const void* pool_d, const ifr_paged_query* q);

@@ -29,7 +29,11 @@ namespace {
 
 constexpr int64_t kMaxRows = 1 << 24;      // rows of a batch
 constexpr int64_t kMaxTokens = 1 << 30;    // tokens of a sequence
-constexpr int64_t kMaxUnits = 1 << 24;     // attention tiles of all kv heads
+constexpr int64_t kMaxStride = (int64_t)1 << 32;
+constexpr int64_t kMaxUnits = 1 << 22;     // attention tiles of all kv heads (a launch has fewer than 2^32 threads)
+
+// scale, cap and scale / cap: products with log2 e and a zero score stay finite.
+constexpr float kMaxFactor = 1e30f;
 
 // Kinds of attention unit, by the columns and the waves of their workgroups:
 // narrow ones of one and two column tiles, wide ones, and narrow ones of two
@@ -244,7 +248,7 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
     if (n == 0 || (n > kWidth[1] && use_wide)) continue;
     cut(n <= kWidth[0] ? 0 : 1, s, tiles);
   }
-  if ((int64_t)tiles.size() * c.n_kv > kMaxUnits || (int64_t)runs.size() * c.n_kv > kMaxTokens)
+  if ((int64_t)tiles.size() * c.n_kv > kMaxUnits || (int64_t)runs.size() * c.n_kv >= 4 * kMaxUnits)
     return fail(IFR_EINVAL, "%lld rows of %d kv heads are too many for one batch", (long long)M, c.n_kv);
   int64_t pages[kKinds] = {}, n_tiles[kKinds] = {}, most[kKinds] = {};
   for (const Tile& t : tiles) {
@@ -404,7 +408,7 @@ ifrk::PagedPool pool_of(const ifr_paged* p, const void* pool) {
 // Rows of `width` elements of `size` bytes: not null, on 16 bytes, wide enough.
 int rows_ok(const char* name, const void* d, int64_t stride, int64_t width, int size) {
   if (!d) return fail(IFR_EINVAL, "%s is null", name);
-  if (!aligned(d, 16) || stride < width || stride * size % 16 != 0 || stride > ((int64_t)1 << 40))
+  if (!aligned(d, 16) || stride < width || stride * size % 16 != 0 || stride > kMaxStride)
     return fail(IFR_EINVAL, "%s: rows of %lld elements need 16-byte alignment and a stride that keeps it (stride %lld)",
                 name, (long long)width, (long long)stride);
   return IFR_OK;
@@ -503,6 +507,9 @@ int ifr_paged_append(ifr_paged* p, void* pool_d, const ifr_paged_rows* r) {
         overlap(r->q_out_d, r->q_out_stride * 2, qw * 2, r->v_d, r->v_stride * 2, kw * 2, p->M) ||
         overlap(pool_d, pb, pb, r->q_out_d, pb, (p->M - 1) * r->q_out_stride * 2 + qw * 2, 1))
       return fail(IFR_EINVAL, "q_out_d overlaps k_d, v_d or the pool");
+    const int64_t tb = (int64_t)r->max_pos * (r->rotary / 2) * 4, ob = (p->M - 1) * r->q_out_stride * 2 + qw * 2;
+    if (r->rotary && (overlap(r->q_out_d, ob, ob, r->cos_d, tb, tb, 1) || overlap(r->q_out_d, ob, ob, r->sin_d, tb, tb, 1)))
+      return fail(IFR_EINVAL, "q_out_d overlaps the rotation's tables");
   }
   OnDevice od(p->device);
   if (int e = note_capture(p)) return e;
@@ -537,9 +544,9 @@ int ifr_paged_attention(ifr_paged* p, const void* pool_d, const ifr_paged_query*
   if (int e = begin(p, pool_d)) return e;
   if (!q) return fail(IFR_EINVAL, "query is null");
   const ifr_paged_cfg& c = p->cfg;
-  if (!(q->scale >= 0.0f) || !std::isfinite(q->scale)) return fail(IFR_EINVAL, "scale %g", q->scale);
+  if (!(q->scale >= 0.0f && q->scale <= kMaxFactor)) return fail(IFR_EINVAL, "scale %g", q->scale);
   const float scale = q->scale > 0.0f ? q->scale : 1.0f / std::sqrt((float)c.head_dim);
-  if (!(q->softcap >= 0.0f) || !std::isfinite(q->softcap) || (q->softcap > 0.0f && !std::isfinite(scale / q->softcap)))
+  if (!(q->softcap >= 0.0f && q->softcap <= kMaxFactor) || (q->softcap > 0.0f && !(scale / q->softcap <= kMaxFactor)))
     return fail(IFR_EINVAL, "softcap %g", q->softcap);
   if (q->out_f32 != 0 && q->out_f32 != 1) return fail(IFR_EINVAL, "out_f32 %d", q->out_f32);
   if (p->M == 0) return IFR_OK;
@@ -550,6 +557,9 @@ int ifr_paged_attention(ifr_paged* p, const void* pool_d, const ifr_paged_query*
   if (overlap(q->out_d, q->out_stride * os, w * os, q->q_d, q->q_stride * 2, w * 2, p->M) ||
       overlap(pool_d, pb, pb, q->out_d, pb, (p->M - 1) * q->out_stride * os + w * os, 1))
     return fail(IFR_EINVAL, "out_d overlaps q_d or the pool");
+  if (const int64_t ob = (p->M - 1) * q->out_stride * os + w * os;
+      q->slopes_d && overlap(q->out_d, ob, ob, q->slopes_d, 4 * c.n_heads, 4 * c.n_heads, 1))
+    return fail(IFR_EINVAL, "out_d overlaps the slopes");
   OnDevice od(p->device);
   if (int e = note_capture(p)) return e;
   ifrk::PagedAttnArgs a{};

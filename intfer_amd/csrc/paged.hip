@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const PagedRun* runs, u
   }
 }
 
-constexpr int64_t kMaxBlocks = 0x7FFFFFFF;
+constexpr int64_t kMaxBlocks = 0xFFFFFF;  // of 256 threads
 
 template <int HD, int FMT>
 hipError_t append_fmt(const PagedAppendArgs& a, const PagedPool& kv, hipStream_t st) {

@@ -763,6 +763,7 @@ def paged_rows():
         case(fmt, 4, 2, 128, [1, 2, 1, 5], [1, 33, 64, 170])
         case(fmt, 2, 2, 64, [1, 3], [95, 40], out_f32=True, rotary=32)
         case(fmt, 8, 2, 256, [1, 4], [31, 67], cap=5.0, rotary=64)
+    case(0, 71, 1, 64, [1, 2], [40, 70], cap=1e-29, scale=1.0)
     case(2, 5, 1, 128, [3, 0, 1], [300, 40, 700], bias=True, prefix=[290, 0, 5], out_f32=True)
     case(0, 3, 1, 64, [7, 6], [7, 50], cap=30.0, rotary=0,
          first=np.array([0, 0, 2, 2, 9, 5, 5, 44, 44, 47, 47, 49, 50]))

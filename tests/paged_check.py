@@ -160,12 +160,14 @@ def refusals(ia, dev):
                  dict(q_out_stride=516), dict(cos=None), dict(sin=None), dict(cos=P(a + 32772)), dict(sin=P(a + 40964)), dict(rotary=8), dict(rotary=144),
                  dict(rotary=-16), dict(max_pos=39), dict(q_out=P(a + 8192 + 16)), dict(q_out=P(a)),
                  dict(q_out=P(a + 4096)), dict(k=P(pool.p.value)), dict(v=P(pool.p.value + 4096)),
-                 dict(q_out=P(pool.p.value))):
+                 dict(q_out=P(pool.p.value)), dict(q_out=P(a + 32768)), dict(q_out=P(a + 40960)), dict(k_stride=1 << 33),
+                 dict(q_out_stride=1 << 33)):
         assert L.ifr_paged_append(plan.h, pool.p, rows(**over)) == I, over
     for over in (dict(q=None), dict(out=None), dict(q=P(a + 8)), dict(out=P(a + 32776)), dict(q_stride=511),
                  dict(q_stride=504), dict(out_stride=508), dict(out_f32=2), dict(scale=-1.0), dict(scale=float("nan")),
                  dict(scale=float("inf")), dict(softcap=-1.0), dict(softcap=float("inf")), dict(softcap=float("nan")),
-                 dict(softcap=1e-44),
+                 dict(softcap=1e-44), dict(softcap=1e-32), dict(softcap=1e31), dict(scale=1e31),
+                 dict(slopes=P(a + 32768)), dict(slopes=P(a + 32768 + 1024)), dict(out_stride=1 << 33),
                  dict(out=P(a)), dict(out=P(a + 1024)), dict(out=P(pool.p.value + 64))):
         assert L.ifr_paged_attention(plan.h, pool.p, query(**over)) == I, over
     for k, v in ((None, P(a)), (P(a), None), (P(a + 2), P(a + 4096)), (P(a), P(a + 256)), (P(a), P(pool.p.value))):

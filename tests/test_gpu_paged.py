@@ -26,6 +26,9 @@ FMT = [ia.KV_FP16, ia.KV_INT8, ia.KV_INT4]
     (9, 3, 64, [7, 0, 2], [50, 90, 35], {"rotary": 32}),          # a sequence that takes no part
     (12, 1, 128, [3, 1], [400, 7], {"scale": 0.25}),              # one kv head
     (32, 1, 64, [1, 2], [77, 64], {"rotary": 0}),                 # 32 columns from one row
+    (71, 1, 128, [1, 3], [500, 40], {"cap": 20.0}),               # more: a row's heads over several tiles
+    (192, 1, 64, [2], [333], {"bias": True, "out_f32": True}),
+    (3, 3, 256, [1, 1, 1], [200, 5, 64], {"prefix": [0, 5, 64]}),  # a head each
 ])
 def test_formats_and_shapes(dev, fmt, nq, nkv, hd, rows, lens, more):
     announce(f"paged fmt={fmt} {nq}/{nkv}x{hd} rows={rows} lens={lens} {more}")
@@ -59,7 +62,8 @@ def test_masks(dev, fmt, rows, lens):
 
 
 @pytest.mark.parametrize("rows,lens", [([1, 4], [400, 77]), ([300], [1700])])
-@pytest.mark.parametrize("cap,scale", [(0.7, 0.3), (3.0, 0.0), (1e4, 0.0), (2e6, 0.1), (50.0, 40.0), (1e-3, 1.0)])
+@pytest.mark.parametrize("cap,scale", [(0.7, 0.3), (3.0, 0.0), (1e4, 0.0), (2e6, 0.1), (50.0, 40.0), (1e-3, 1.0),
+                                       (1e-29, 1.0), (1e30, 0.0)])
 def test_caps(dev, rows, lens, cap, scale):
     """Caps that scores never come near, that all of them are far beyond, and both sides of where the polynomial and
     the exponential share the work."""
