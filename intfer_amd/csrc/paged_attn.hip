@@ -321,14 +321,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedJoin* joins,
     m = mr;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (s0 + k >= j.ns || q[k].x == -INFINITY) continue;
+      if (s0 + k >= j.ns) continue;  // (a split without a finite score: 0, or a NaN that is to stay)
       const float f = __builtin_amdgcn_exp2f(q[k].x - mu);
       l += f * q[k].y;
       x += p[k] * f;
     }
   }
-  x *= l == 0.0f ? 0.0f : 1.0f / l;
   const int G = kv.nq / kv.nkv, col = j.col0 + i;
+  const PagedRow row = a.rows[j.row0 + col / G];
+  x *= l != 0.0f ? 1.0f / l : row.lo < row.hi ? NAN : 0.0f;
   const int64_t at = (int64_t)(j.row0 + col / G) * a.out_stride + (int64_t)(j.kvh * G + col % G) * HD + d;
   if (a.out_f32)
     *reinterpret_cast<v4f*>(static_cast<float*>(a.out) + at) = x;
@@ -588,7 +589,8 @@ __global__ __launch_bounds__(64 * NW, paged_narrow_waves(FMT, HD, NT)) void page
     for (int q = 0; q < NW; ++q) l += __builtin_amdgcn_exp2f(ml[q][16 * t + c][0] - mu) * ml[q][16 * t + c][1];
     f[t] = __builtin_amdgcn_exp2f(m_run[t] - mu);
     if (un.part < 0) {
-      f[t] = l == 0.0f ? 0.0f : f[t] / l;  // a row that sees nothing: zeros
+      // a row that sees nothing: zeros; only scores of -infinity: not a number
+      f[t] = l != 0.0f ? f[t] / l : lo[t] < hi[t] ? NAN : 0.0f;
     } else if (w == 0 && g == 0 && on[t]) {
       float* p = a.part_ml + ((int64_t)un.part + 16 * t + c) * 2;
       p[0] = m;
@@ -895,7 +897,7 @@ __global__ __launch_bounds__(256, kPgWideGroups) void paged_wide_kernel(PagedAtt
   if (!on) return;
   float f = 1.0f;
   if (un.part < 0) {
-    f = l == 0.0f ? 0.0f : 1.0f / l;
+    f = l != 0.0f ? 1.0f / l : lo < hi ? NAN : 0.0f;
   } else if (hl == 0) {
     float* p = a.part_ml + ((int64_t)un.part + ci) * 2;
     p[0] = m_run;

@@ -778,6 +778,7 @@ def paged_chunks():
     case = lambda *a, **k: run_case(ia, dev, rng, *a, **k, say=say)  # noqa: E731
     for fmt in (0, 1, 2):
         case(fmt, 2, 1, 128, [70, 1], [101, 9], cap=9.0)
+        case(fmt, 2, 1, 128, [99, 2], [500, 70], cap=9.0, bias=fmt == 1, out_f32=fmt != 1, prefix=[480, 0])  # eight waves
         case(fmt, 1, 1, 64, [140], [300], out_f32=True)
         case(fmt, 3, 1, 256, [12, 40], [12, 75], bias=True)
     pos = np.arange(90, 140)

@@ -193,6 +193,56 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(dev, rows, lens, nkv, va
     plan.close()
 
 
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("rows,lens,nkv", [([1, 3, 5], [70, 80, 900], 2), ([100], [150], 2), ([130], [500], 8),
+                                           ([260, 260], [400, 500], 64)])
+def test_queries_that_are_not_finite_stay_in_their_rows(dev, rows, lens, nkv, value):
+    for fmt, cap in ((ia.KV_FP16, 0.0), (ia.KV_INT4, 20.0)):
+        announce(f"paged query {value} rows={rows} fmt={fmt}")
+        nq, hd = 2 * nkv, 128
+        cache, table, plan, q, pool, _, out = _setup(dev, fmt, nq, nkv, hd, rows, lens)
+        want, tol = pr.expect(cache, rows, lens, table, q, cap=cap, out_f32=True)
+        bad = np.zeros(q.shape[:2], bool)
+        bad[len(q) // 2, 1] = bad[-1, nq - 1] = True
+        q[bad] = value
+        qd = dev.upload(q)
+        plan.set(rows, lens, table)
+        plan.attention(pool.p, qd.p, out.p, out_f32=True, softcap=cap)
+        got = dev.download(out, np.float32, q.shape).astype(np.float64)
+        assert (np.abs(got - want)[~bad] <= tol[~bad]).all()
+        if np.isnan(value):
+            assert np.isnan(got[bad]).all()
+        plan.close()
+
+
+@pytest.mark.parametrize("rows,lens,nkv", [([1, 3, 5], [1, 80, 900], 2), ([100], [150], 2), ([130], [500], 8),
+                                           ([260, 260], [400, 500], 64)])
+def test_scores_of_minus_infinity_only(dev, rows, lens, nkv):
+    """The softmax of scores that are all -infinity is not a number; a row that sees nothing still gives zeros."""
+    fmt, nq, hd = ia.KV_FP16, 2 * nkv, 128
+
+    def edit(cache, table):
+        cache.pool.view(np.uint16)[..., :] &= 0x7FFF  # values of one sign
+
+    announce(f"paged -inf rows={rows}")
+    cache, table, plan, q, pool, _, out = _setup(dev, fmt, nq, nkv, hd, rows, lens, edit=edit)
+    pos = np.concatenate([np.arange(n - r, n) for r, n in zip(rows, lens)])
+    first = np.where(np.arange(len(pos)) % 7 == 3, pos + 1, 0)
+    bad = np.zeros(q.shape[:2], bool)
+    bad[::3, 1] = bad[-1, nq - 1] = True
+    want, tol = pr.expect(cache, rows, lens, table, q, first, out_f32=True)
+    q[bad] = 0
+    q[bad, 5] = -np.inf
+    qd = dev.upload(q)
+    plan.set(rows, lens, table, first=first)
+    plan.attention(pool.p, qd.p, out.p, out_f32=True)
+    got = dev.download(out, np.float32, q.shape).astype(np.float64)
+    assert (np.abs(got - want)[~bad] <= tol[~bad]).all()
+    blind = first > pos
+    assert np.isnan(got[bad & ~blind[:, None]]).all() and (got[blind] == 0).all()
+    plan.close()
+
+
 @pytest.mark.parametrize("fmt", [ia.KV_INT8, ia.KV_INT4])
 @pytest.mark.parametrize("rows,lens,nkv", [([1, 3], [70, 80], 2), ([100], [150], 2), ([130], [500], 8), ([260, 260], [400, 500], 64)])
 def test_quantized_rows_without_a_scale(dev, fmt, rows, lens, nkv):
