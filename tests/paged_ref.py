@@ -100,24 +100,25 @@ def quantize(x, fmt):
         return c.reshape(x.shape), rep(s), rep(z)
 
 
-def write_token(part, fmt, hd, v, t, x):
-    """Store one token's row x (fp32 [hd]) in a part, in place."""
-    c, s, z = quantize(x[None], fmt)
+def write_token(parts, fmt, hd, v, t, x):
+    """Store one token's rows x (fp32 [n_kv, hd]) in its heads' parts (uint8 [n_kv, bytes]), in place."""
+    c, s, z = quantize(x, fmt)
     e = element(fmt, hd, v)[t]
     if fmt == FP16:
-        part.view(np.float16)[e] = c[0]
+        parts.view(np.float16)[:, e] = c
         return
     i, off = scale_index(fmt, hd, v)
-    sc = part[(32 if fmt == INT8 else 16) * hd:].view(np.float16)
-    sc[i[t]] = s[0]
+    k = (32 if fmt == INT8 else 16) * hd
+    sc = parts[:, k:].view(np.float16)
+    sc[:, i[t]] = s
     if fmt == INT8:
-        part[:32 * hd].view(np.int8)[e] = c[0]
+        parts[:, :k].view(np.int8)[:, e] = c
         return
-    sc[i[t] + off] = z[0]
+    sc[:, i[t] + off] = z
     nib = e // 8 * 8 + 4 * (e % 2) + e % 8 // 2
     lo, hi = nib % 2 == 0, nib % 2 == 1
-    part[nib[lo] // 2] = (part[nib[lo] // 2] & 0xF0) | c[0, lo]
-    part[nib[hi] // 2] = (part[nib[hi] // 2] & 0x0F) | (c[0, hi] << 4)
+    parts[:, nib[lo] // 2] = (parts[:, nib[lo] // 2] & 0xF0) | c[:, lo]
+    parts[:, nib[hi] // 2] = (parts[:, nib[hi] // 2] & 0x0F) | (c[:, hi] << 4)
 
 
 def tables(max_pos, rotary, theta=1e6):
@@ -173,9 +174,8 @@ class Cache:
 
     def append(self, pages, pos, k, v):
         """Row (fp32 [n_kv, hd]) at position pos."""
-        for h in range(self.n_kv):
-            for w, x in ((0, k), (1, v)):
-                write_token(self.pool[pages[pos // PAGE], h, w], self.fmt, self.hd, w, pos % PAGE, x[h])
+        for w, x in ((0, k), (1, v)):
+            write_token(self.pool[pages[pos // PAGE], :, w], self.fmt, self.hd, w, pos % PAGE, x)
 
 
 def attention(q, k, v, pos, lo, hi, scale, cap, slopes, out_f32):
