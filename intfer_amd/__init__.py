@@ -439,6 +439,14 @@ class Engine:
         return ms.value, n.value, b.value, f.value
 
 
+def _int32(x):
+    a = np.asarray(x)
+    i = np.ascontiguousarray(a, dtype=np.int32)
+    if a.size and (a.dtype.kind not in "iu" or not np.array_equal(i, a)):
+        raise ValueError("batch entries are 32-bit whole numbers")
+    return i
+
+
 class Paged:
     """The plan of a paged KV cache that the caller owns (ifr_paged_*): device
     pointers are integers or c_void_p, strides count elements."""
@@ -455,7 +463,7 @@ class Paged:
         """Per sequence: new rows, cached tokens (the new ones among them) and the
         pages; optionally the first visible position of each row and a prefix of
         each sequence."""
-        a = [None if x is None else np.ascontiguousarray(x, dtype=np.int32) for x in (rows, lens, table, first, prefix)]
+        a = [None if x is None else _int32(x) for x in (rows, lens, table, first, prefix)]
         S = len(a[0])
         if len(a[1]) != S or a[2].ndim != 2 or a[2].shape[0] != S or (a[4] is not None and len(a[4]) != S):
             raise ValueError("rows, lens, table and prefix name different numbers of sequences")

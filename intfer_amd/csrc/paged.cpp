@@ -321,7 +321,8 @@ int set_batch(ifr_paged* p, const ifr_paged_batch* b) {
       if (cols > kMaxTokens) return fail(IFR_EINVAL, "too many partial columns");
       for (int h = 0; h < c.n_kv; ++h)
         for (int i = 0, n = 1024 / c.head_dim; i < t.ncol; i += n)
-          joins.push_back({row0[t.seq], h, t.col0 + i, std::min(n, t.ncol - i), (int)(base + (int64_t)h * ns * t.ncol) + i, t.ncol, ns, 0});
+          joins.push_back({row0[t.seq], h, t.col0 + i, std::min(n, t.ncol - i),
+                           (int)(base + (int64_t)h * ns * t.ncol) + i, t.ncol, ns, 0});
     }
   }
   // the longest first, for short ones to fill the end

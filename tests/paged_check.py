@@ -144,6 +144,13 @@ def refusals(ia, dev):
     assert bad_set([41, 1], [40, 33], t) == I         # more new rows than tokens
     assert bad_set([1, 1], [40, 33], t, prefix=[0, -1]) == I
     assert L.ifr_paged_set(plan.h, None) == I and L.ifr_paged_set(None, C.byref(_abi.PagedBatch())) == I
+    for r, n, tb in (([1, 1], [40, 33], t.astype(np.int64) + 2**32), ([1, 1], [40, 2**32 + 33], t), ([1.5, 1], [40, 33], t),
+                     ([1], [40, 33], t), ([1, 1], [40, 33], t[0])):
+        try:
+            plan.set(r, n, tb)
+        except ValueError:
+            continue
+        raise AssertionError((r, n, tb))
     # a sequence without new rows takes no part, whatever stands in its entries
     assert bad_set([1, 0], [40, -3], np.array([[0, 1], [99, -7]])) == ia.IFR_OK
     assert bad_set([], [], np.zeros((0, 0))) == ia.IFR_OK  # an empty batch: calls do nothing
@@ -157,8 +164,8 @@ def refusals(ia, dev):
     plan.set([2, 1], [40, 33], t)
     for over in (dict(k=None), dict(v=None), dict(k=P(a + 2)), dict(v=P(a + 4104)), dict(k_stride=255), dict(k_stride=248),
                  dict(v_stride=260), dict(q=None), dict(q_out=None), dict(q=P(a + 8200)), dict(q_stride=504),
-                 dict(q_out_stride=516), dict(cos=None), dict(sin=None), dict(cos=P(a + 32772)), dict(sin=P(a + 40964)), dict(rotary=8), dict(rotary=144),
-                 dict(rotary=-16), dict(max_pos=39), dict(q_out=P(a + 8192 + 16)), dict(q_out=P(a)),
+                 dict(q_out_stride=516), dict(cos=None), dict(sin=None), dict(cos=P(a + 32772)),
+                 dict(sin=P(a + 40964)), dict(rotary=8), dict(rotary=144), dict(rotary=-16), dict(max_pos=39), dict(q_out=P(a + 8192 + 16)), dict(q_out=P(a)),
                  dict(q_out=P(a + 4096)), dict(k=P(pool.p.value)), dict(v=P(pool.p.value + 4096)),
                  dict(q_out=P(pool.p.value)), dict(q_out=P(a + 32768)), dict(q_out=P(a + 40960)), dict(k_stride=1 << 33),
                  dict(q_out_stride=1 << 33)):
